@@ -91,6 +91,55 @@ int dsa_linear_pack(const void* w, int N, int K, int G, void* packed, size_t pac
 
 /* ---------------------------------------------------------------- attn.kv */
 
+/* MXFP4 (OCP microscaling) quantisation of x [M, K] (row stride ld_x) along
+ * K, blocks of 32: e = floor(log2(max |x|)) - 2 clamped to [-127, 127], scale
+ * code e + 127 (UE8M0), element = E2M1 nearest to x 2^-e, ties to even,
+ * saturating at 6.  A block of zeros takes code 0; one that holds a NaN or an
+ * infinity takes code 255 (NaN) and zero elements.
+ * codes [M, K/2]: two elements a byte, the even one in the low half; scales
+ * [M, K/32]; both contiguous.  out [M, K] of x's type, row stride ld_out (may
+ * be NULL; may be x): the values the codes stand for, NaN in a block of code
+ * 255.  K a multiple of 32; x and out 16-byte aligned, their row strides
+ * multiples of 16 bytes.
+ * The 4-bit counterpart of dsa_act_quant_block; the reference reads such
+ * weights (inference.py:283-327) and expands them. */
+enum { DSA_BF16 = 0, DSA_FP16 = 1, DSA_FP32 = 2 };
+int dsa_mxfp4_quant(const void* x, int x_type, int64_t ld_x, void* out, int64_t ld_out, uint8_t* codes,
+                    uint8_t* scales, int64_t M, int64_t K, dsa_stream_t stream);
+
+/* The FP8 latent cache: rows of D dims, the last rope_dim rotary, as records
+ *   [D - rope_dim e4m3 codes][rope_dim bf16][(D - rope_dim) / 64 fp32 scales][0 ..]
+ * of dsa_kv_quant_row_bytes(D, rope_dim) bytes, a multiple of 32 (608 for
+ * D = 512, rope_dim = 64; 0 for sizes that are not built: D - rope_dim must
+ * be a positive multiple of 64, rope_dim a multiple of 8, D <= 8192). */
+size_t dsa_kv_quant_row_bytes(int D, int rope_dim);
+
+/* Quantises rows of kv [B, S, D] bf16 (strides ld_b, ld_s elements, multiples
+ * of 8; unit stride in D) as it writes them: token s < n_valid[b] (NULL: S) of
+ * sequence b goes to record offset + (pos[b] + s) % win of its cache rows
+ * [cache_rows, row bytes] at cache + b * cache_bstride bytes.  win = the ring's
+ * length (kv_window_write's window; the rows behind it for a cache that does
+ * not wrap).  Of more than win tokens the last win are written, so a call
+ * writes no record twice; tokens at negative positions are skipped, all other
+ * records stay as they were.
+ * Per 64 dims: s = max(max |x|, 1e-4) * fl(1/448), code = e4m3_rn(x / s); the
+ * rotary dims keep their bf16 bits.  A block that holds a NaN or an infinity
+ * takes a NaN scale and zero codes.  Same arithmetic as dsa_kv_window_write
+ * (inference.py:4578-4607, 6072-6079) for finite rows. */
+int dsa_kv_quant_write(const void* kv, int64_t ld_b, int64_t ld_s, void* cache, int64_t cache_bstride,
+                       int64_t cache_rows, const int32_t* pos, const int32_t* n_valid, int B, int S, int D,
+                       int rope_dim, int win, int64_t offset, dsa_stream_t stream);
+
+/* Reads records back: out [B, K, D] contiguous, bf16 - bf16(code * scale) and
+ * the rotary bits, what dsa_kv_window_write stores for the same finite row -
+ * or, with out_f32, the fp32 product itself.  idx [B, K] int32 (row stride
+ * ld_idx): records by number, negative ones read as zero rows, those >=
+ * cache_rows are clamped and set status bit 1 (status may be NULL).  idx NULL:
+ * the first K records. */
+int dsa_kv_quant_read(const void* cache, int64_t cache_bstride, int64_t cache_rows, const int32_t* idx,
+                      int64_t ld_idx, void* out, int out_f32, int B, int64_t K, int D, int rope_dim, int32_t* status,
+                      dsa_stream_t stream);
+
 /* Block-wise max-abs FP8-E4M3 round trip of an [M, N] bf16 matrix along N.
  * Per block of `block` columns: amax = max|x|; s = max(amax, eps) * r where
  * r = 1/fp8_max rounded to fp32 (the chain multiplies by the constant, it
@@ -491,6 +540,20 @@ int dsa_sparse_attn_ex(const void* q, const void* kv, int64_t kv_bstride, int64_
                        float* lse, int B, int S, int H, int D, int K, float scale,
                        void* workspace, size_t workspace_bytes, int lead_cols, unsigned flags,
                        int32_t* status, dsa_stream_t stream);
+
+/* dsa_sparse_attn over the FP8 latent cache: cache holds records of
+ * dsa_kv_quant_row_bytes(512, 64) = 608 bytes, cache_rows a sequence,
+ * sequences cache_bstride bytes apart (a multiple of 16); each selected
+ * record is expanded to its bf16 row on the way into the tensor cores, so the
+ * result is dsa_sparse_attn's over the rows that dsa_kv_quant_read returns,
+ * for 0.59 of the bytes.  Everything else (masks, sink, lse, status,
+ * workspace of dsa_sparse_attn_workspace_size bytes) as there; B*S <= 65535.
+ * Replaces the same reference stage (inference.py:4459-4501), which has no
+ * 8-bit cache. */
+int dsa_sparse_attn_quant(const void* q, const void* cache, int64_t cache_bstride, int64_t cache_rows,
+                          const int32_t* idx, int64_t ld_idx, const float* sink, void* out, float* lse, int B, int S,
+                          int H, int D, int K, float scale, void* workspace, size_t workspace_bytes, int32_t* status,
+                          dsa_stream_t stream);
 
 /* Allocation-free variant of dsa_sparse_attn, for callers that cannot
  * allocate device memory where they call the attention (a runtime that owns

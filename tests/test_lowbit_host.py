@@ -1,0 +1,156 @@
+"""The low-bit operators without a GPU: the 64-bit forms the GPU tests compare
+with, sizes that are host arithmetic, and every refusal - none of these calls
+reaches a launch."""
+
+import pytest
+import torch
+
+import lowbit
+
+BF, I32 = torch.bfloat16, torch.int32
+
+
+def test_mxfp4_reference_values():
+    x = torch.zeros(1, 64)
+    x[0, :8] = torch.tensor([7.9, 0.25, 0.75, 2.5, -3.5, 5.0, 1.0, -0.1])
+    x[0, 32] = 1e-40
+    code, sc, val = lowbit.mxfp4(x)
+    assert sc.tolist() == [[127, 0]]                       # floor(log2 7.9) - 2 = 0; below 2^-124: code 0
+    # 7.9 saturates; ties 0.25, 0.75, 2.5, 3.5, 5 go to the even code
+    assert val[0, :8].tolist() == [6.0, 0.0, 1.0, 2.0, -4.0, 4.0, 1.0, -0.0]
+    assert code[0, :8].tolist() == [7, 0, 2, 4, 14, 6, 2, 8]
+    assert torch.equal(lowbit.mxfp4_values(lowbit.pack_nibbles(code), sc), val)
+
+
+def test_mxfp4_reference_non_finite_block():
+    x = torch.ones(1, 64)
+    x[0, 3] = float("inf")
+    code, sc, val = lowbit.mxfp4(x)
+    assert sc.tolist() == [[255, 125]] and bool(val[0, :32].isnan().all()) and not bool(val[0, 32:].isnan().any())
+
+
+def test_record_bytes():
+    from dsv4attn import ops
+    from dsv4attn import _lib
+    assert ops.kv_quant_row_bytes(512, 64) == 608          # 448 + 128 + 28, up to a multiple of 32
+    assert ops.kv_quant_row_bytes(128, 0) == 160
+    assert ops.kv_quant_row_bytes(96, 32) == 160
+    for D, r in ((512, 60), (512, 512), (500, 64), (0, 0), (8256, 64), (64, -8)):
+        assert _lib.lib().dsa_kv_quant_row_bytes(D, r) == 0
+        with pytest.raises(ValueError, match="multiple"):
+            ops.kv_quant_row_bytes(D, r)
+
+
+def test_cache_views():
+    from dsv4attn import ops
+    cache = ops.kv_quant_cache(2, 5, device="cpu")
+    codes, rope, scales = ops.kv_quant_views(cache)
+    assert codes.shape == (2, 5, 448) and rope.shape == (2, 5, 64) and scales.shape == (2, 5, 7)
+    scales[1, 4, 6] = 1.0
+    rope[1, 4, 0] = 1.0
+    assert cache[1, 4, 448:450].view(BF).item() == 1.0 and cache[1, 4, 600:604].view(torch.float32).item() == 1.0
+    with pytest.raises(ValueError, match="608"):
+        ops.kv_quant_views(torch.zeros(2, 5, 600, dtype=torch.uint8))
+
+
+def test_ops_refuse_cpu_tensors():
+    from dsv4attn import ops
+    cache = ops.kv_quant_cache(1, 8, device="cpu")
+    pos = torch.zeros(1, dtype=I32)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.mxfp4_quant(torch.zeros(2, 64))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.kv_quant_write(torch.zeros(1, 512, dtype=BF), cache, pos, 8)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.kv_quant_read(cache)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.sparse_attn_quant(torch.zeros(1, 64, 512, dtype=BF), cache, torch.zeros(1, 4, dtype=I32), torch.zeros(64), 0.1)
+
+
+# --------------------------------------------------- refusals of the C entries
+# pointers are 16-byte-aligned numbers that nothing reads: every call returns
+# before it touches the GPU
+
+def _refused(rc, *words):
+    from dsv4attn import _lib
+    assert rc == _lib.DSA_ERR_ARG, rc
+    msg = _lib.last_error()
+    assert all(w in msg for w in words), msg
+
+
+def test_mxfp4_quant_refusals():
+    from dsv4attn import _lib
+    f = _lib.lib().dsa_mxfp4_quant
+    _refused(f(None, 0, 64, None, 0, 16, 16, 1, 64, None), "null")
+    _refused(f(16, 0, 64, None, 0, None, 16, 1, 64, None), "null")
+    _refused(f(16, 3, 64, None, 0, 16, 16, 1, 64, None), "x_type")
+    _refused(f(16, 0, 48, None, 0, 16, 16, 1, 48, None), "32")
+    _refused(f(16, 0, 64, None, 0, 16, 16, -1, 64, None), "M/K")
+    _refused(f(16, 0, 32, None, 0, 16, 16, 1, 64, None), "stride")
+    _refused(f(16, 0, 68, None, 0, 16, 16, 2, 64, None), "16 bytes")
+    _refused(f(8, 0, 64, None, 0, 16, 16, 1, 64, None), "alignment")
+    _refused(f(16, 0, 64, 8, 64, 16, 16, 1, 64, None), "out")
+    _refused(f(16, 0, 64, None, 0, 18, 16, 1, 64, None), "codes")
+    assert f(16, 0, 64, None, 0, 16, 16, 0, 64, None) == _lib.DSA_OK
+
+
+def test_kv_quant_write_refusals():
+    from dsv4attn import _lib
+    f = _lib.lib().dsa_kv_quant_write
+    ok = dict(kv=16, ld_b=512, ld_s=512, cache=16, bs=608 * 8, rows=8, pos=16, n=None, B=2, S=1, D=512, r=64, win=8,
+              off=0, st=None)
+
+    def call(**kw):
+        return f(*{**ok, **kw}.values())
+    _refused(call(kv=None), "null")
+    _refused(call(pos=None), "null")
+    _refused(call(r=60), "multiple of 64")
+    _refused(call(D=8256), "8192")
+    _refused(call(rows=0), "rows")
+    _refused(call(bs=608 * 7), "batch stride")
+    _refused(call(bs=608 * 8 + 8), "16-byte")
+    _refused(call(cache=24), "16-byte")
+    _refused(call(win=0), "ring")
+    _refused(call(off=1), "ring")
+    _refused(call(off=-1), "ring")
+    _refused(call(kv=18), "kv needs")
+    _refused(call(ld_s=516), "kv needs")
+    _refused(call(B=-1), "B/rows")
+    assert call(B=0) == _lib.DSA_OK and call(S=0) == _lib.DSA_OK
+
+
+def test_kv_quant_read_refusals():
+    from dsv4attn import _lib
+    f = _lib.lib().dsa_kv_quant_read
+    ok = dict(cache=16, bs=608 * 8, rows=8, idx=16, ld=4, out=16, f32=0, B=2, K=4, D=512, r=64, status=None, st=None)
+
+    def call(**kw):
+        return f(*{**ok, **kw}.values())
+    _refused(call(cache=None), "null")
+    _refused(call(out=None), "null")
+    _refused(call(ld=3), "ld_idx")
+    _refused(call(idx=None, K=9), "more rows")
+    _refused(call(out=24), "aligned")
+    _refused(call(D=500), "multiple of 64")
+    _refused(call(K=-1), "K")
+    assert call(B=0) == _lib.DSA_OK and call(K=0) == _lib.DSA_OK
+
+
+def test_sparse_attn_quant_refusals():
+    from dsv4attn import _lib
+    f = _lib.lib().dsa_sparse_attn_quant
+    ok = dict(q=16, cache=16, bs=608 * 8, rows=8, idx=16, ld=4, sink=16, out=16, lse=None, B=2, S=1, H=64, D=512, K=4,
+              scale=1.0, ws=None, wsb=0, status=None, st=None)
+
+    def call(**kw):
+        return f(*{**ok, **kw}.values())
+    _refused(call(q=None), "null")
+    _refused(call(sink=None), "null")
+    _refused(call(H=32), "H=64")
+    _refused(call(D=576), "D=512")
+    _refused(call(bs=608 * 7), "stride")
+    _refused(call(bs=608 * 8 + 8), "stride")
+    _refused(call(ld=3), "ld_idx")
+    _refused(call(q=24), "aligned")
+    _refused(call(B=32768, S=2), "65535")
+    assert call(B=0) == _lib.DSA_OK

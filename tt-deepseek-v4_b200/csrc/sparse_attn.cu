@@ -169,21 +169,28 @@ static void ensure_attr() {
   int dev = 0;
   cudaGetDevice(&dev);
   if (done_dev != dev) {
-    cudaFuncSetAttribute(satc::sparse_attn_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         satc::kSmemBytes);
-
+    for (auto k : {satc::sparse_attn_tc_kernel<false>, satc::sparse_attn_tc_kernel<true>})
+      cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, satc::kSmemBytes);
     done_dev = dev;
   }
 }
 
+// quant: kv holds records of the FP8 latent cache and kv_bstride is in bytes
 static int check_common(const void* q, const void* kv, int64_t kv_bstride, int64_t kv_rows, const int32_t* idx,
-                        int64_t ld_idx, int B, int S, int H, int D, int K) {
+                        int64_t ld_idx, int B, int S, int H, int D, int K, bool quant) {
   DSA_CHECK_ARG(q && kv && idx, "sparse_attn: null q/kv/idx");
   DSA_CHECK_ARG(H == kSaH && D == kSaD, "sparse_attn: built for H=64, D=512 (got H=%d D=%d)", H, D);
   DSA_CHECK_ARG(B >= 0 && S >= 1 && K >= 0 && kv_rows > 0, "sparse_attn: bad B/S/K/kv_rows");
   DSA_CHECK_ARG(int64_t(B) * S <= INT32_MAX / kSaH, "sparse_attn: B*S = %lld query rows is too many",
                 (long long)B * S);
-  DSA_CHECK_ARG(kv_bstride >= kv_rows * D && kv_bstride % 8 == 0, "sparse_attn: bad kv batch stride");
+  if (quant) {
+    DSA_CHECK_ARG(kv_rows <= INT32_MAX && (B <= 1 || kv_bstride >= kv_rows * satc::kRecBytes) && kv_bstride % 16 == 0,
+                  "sparse_attn_quant: bad cache batch stride");
+    DSA_CHECK_ARG(int64_t(B) * S <= 65535, "sparse_attn_quant: B*S = %lld query rows is too many (65535 a call)",
+                  (long long)B * S);
+  } else {
+    DSA_CHECK_ARG(kv_bstride >= kv_rows * D && kv_bstride % 8 == 0, "sparse_attn: bad kv batch stride");
+  }
   DSA_CHECK_ARG(ld_idx >= K, "sparse_attn: ld_idx < K");
   DSA_CHECK_ARG(aligned(q, 16) && aligned(kv, 16), "sparse_attn: q/kv must be 16-byte aligned");
   return DSA_OK;
@@ -206,8 +213,8 @@ static int sparse_attn_run(const void* q, const void* kv, int64_t kv_bstride, in
                            int64_t ld_idx, const float* sink, void* out, float* lse, float* part_ml_out,
                            float* part_o_out, int B, int S, int H, int D, int K, float scale, void* ws,
                            size_t ws_bytes, int32_t* status, cudaStream_t st, bool final_mode, int lead_cols = 0,
-                           unsigned flags = 0) {
-  int rc = check_common(q, kv, kv_bstride, kv_rows, idx, ld_idx, B, S, H, D, K);
+                           unsigned flags = 0, bool quant = false) {
+  int rc = check_common(q, kv, kv_bstride, kv_rows, idx, ld_idx, B, S, H, D, K, quant);
   if (rc) return rc;
   const int M = B * S;
   if (M == 0) return DSA_OK;
@@ -218,7 +225,7 @@ static int sparse_attn_run(const void* q, const void* kv, int64_t kv_bstride, in
                 "sparse_attn: out / part_o must be 16-byte aligned");
   satc::Args t{};
   t.q = static_cast<const __nv_bfloat16*>(q);
-  t.kv = static_cast<const __nv_bfloat16*>(kv);
+  t.kv = kv;
   t.kv_bstride = kv_bstride;
   t.kv_rows = kv_rows;
   t.idx = idx;
@@ -282,8 +289,9 @@ static int sparse_attn_run(const void* q, const void* kv, int64_t kv_bstride, in
     t.part_ml = part_ml_out;
     t.part_o = part_o_out;
   }
-  DSA_CHECK_ARG(kv_bstride % kSaD == 0, "sparse_attn: kv batch stride must be a multiple of D");
-  const int64_t row_stride = kv_bstride / kSaD;
+  DSA_CHECK_ARG(quant || kv_bstride % kSaD == 0, "sparse_attn: kv batch stride must be a multiple of D");
+  const int64_t row_stride = quant ? kv_bstride : kv_bstride / kSaD;
+  auto kernel = quant ? satc::sparse_attn_tc_kernel<true> : satc::sparse_attn_tc_kernel<false>;
   CUtensorMap tm_q;
   if (!tma::make_2d_bf16(&tm_q, q, kSaD, uint64_t(M) * kSaH, kSaD * 2, 64, 64)) {
     set_error("sparse_attn: cuTensorMapEncodeTiled failed");
@@ -304,12 +312,11 @@ static int sparse_attn_run(const void* q, const void* kv, int64_t kv_bstride, in
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    cudaLaunchKernelEx(&cfg, satc::sparse_attn_tc_kernel, t, tm_q, row_stride);
+    cudaLaunchKernelEx(&cfg, kernel, t, tm_q, row_stride);
     DSA_CHECK_LAUNCH("sparse_attn");
     return DSA_OK;
   }
-  launch_pdl(satc::sparse_attn_tc_kernel, dim3(p.nsplit, M), dim3(satc::THREADS), satc::kSmemBytes, st, t, tm_q,
-             row_stride);
+  launch_pdl(kernel, dim3(p.nsplit, M), dim3(satc::THREADS), satc::kSmemBytes, st, t, tm_q, row_stride);
   DSA_CHECK_LAUNCH("sparse_attn");
   if (p.nsplit > 1) {
     launch_lse_combine(ws_ml, ws_o, true, sink, p.nsplit, M, kSaH, kSaD, final_mode ? 1 : 0,
@@ -340,6 +347,17 @@ extern "C" int dsa_sparse_attn(const void* q, const void* kv, int64_t kv_bstride
   DSA_CHECK_ARG(sink && out, "sparse_attn: null sink/out");
   return sparse_attn_run(q, kv, kv_bstride, kv_rows, idx, ld_idx, sink, out, lse, nullptr, nullptr, B, S, H, D, K,
                          scale, workspace, workspace_bytes, status, reinterpret_cast<cudaStream_t>(stream), true);
+}
+
+extern "C" int dsa_sparse_attn_quant(const void* q, const void* cache, int64_t cache_bstride, int64_t cache_rows,
+                                     const int32_t* idx, int64_t ld_idx, const float* sink, void* out, float* lse,
+                                     int B, int S, int H, int D, int K, float scale, void* workspace,
+                                     size_t workspace_bytes, int32_t* status, dsa_stream_t stream) {
+  clear_error();
+  DSA_CHECK_ARG(sink && out, "sparse_attn_quant: null sink/out");
+  return sparse_attn_run(q, cache, cache_bstride, cache_rows, idx, ld_idx, sink, out, lse, nullptr, nullptr, B, S, H,
+                         D, K, scale, workspace, workspace_bytes, status, reinterpret_cast<cudaStream_t>(stream), true,
+                         0, 0, true);
 }
 
 extern "C" int dsa_sparse_attn_partial(const void* q, const void* kv, int64_t kv_bstride, int64_t kv_rows,

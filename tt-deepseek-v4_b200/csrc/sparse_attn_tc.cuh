@@ -56,12 +56,21 @@
 //               rows of Q' into tensor memory (conflict-free ld.shared,
 //               tcgen05.st), after which the slot takes its first tile.
 //
+// kQuant: the rows are records of the FP8 latent cache (kv_quant_dev.cuh).
+// The producers load a record's codes, scales and rotary dims into registers,
+// expand them to the bf16 rows of the tile and store those where the copies
+// of the bf16 cache land; everything behind the tile is the same.  Registers,
+// not a staging ring: the three 64 KB slots leave 3 KB of shared memory.  A
+// warp keeps two groups of four rows, the next group's loads in flight while
+// it expands the one before.
+//
 // Every mbarrier wait is bounded (about a second); a wait that runs out sets
 // a status bit and an abort flag that makes all later waits of the CTA return
 // at once, so a lost arrival ends the launch with an error instead of a hang.
 #pragma once
 
 #include "common.cuh"
+#include "kv_quant_dev.cuh"
 #include "tc05.cuh"
 #include "tma.cuh"
 
@@ -108,10 +117,18 @@ constexpr uint32_t kColS = 384;   // S: [128 Q' rows x 128 tile rows] fp32
 // pair combine exchange per (row, receiving CTA): 32 heads' O^T as
 // [8 chunks][512 dims][4] fp32, then (m, l) of the 32 heads
 constexpr int kPairXFloats = 8 * D * 4 + 64;
+// records of the FP8 cache: 448 codes, 64 rotary bf16, 7 scales
+constexpr int kRope = 64;
+constexpr int kNope = D - kRope;
+constexpr int kRecBytes = kvq::row_bytes(kNope, kRope);
+constexpr int kGroup = 4;                             // rows a producer warp loads at a time (kQuant)
+constexpr int kGroups = 2;                            // groups a tile: kGroup * kGroups * kProducerWarps >= TK
 constexpr uint32_t kIdescS = tc::idesc_bf16(128, 128, false, false);
 constexpr uint32_t kIdescPV = tc::idesc_bf16(128, 64, true, false);
 static_assert(kSmemBytes <= 232448, "shared memory budget");
 static_assert(kColS + 128 <= kTmemCols, "TMEM columns");
+static_assert(kGroup * kGroups * kProducerWarps >= TK, "a producer warp's rows of a tile");
+static_assert(kNope / 8 == 56 && kRope / 8 == 8, "a lane's two chunks of a record: 56 of codes, 8 of rotary dims");
 static_assert(TK == 64, "the block-diagonal layout assumes 64-key tiles");
 static_assert(kIdxCap % 32 == 0 && THREADS % 32 == 0, "index staging ballots whole warps");
 
@@ -119,7 +136,7 @@ enum : int { kStatusBadIndex = 1, kStatusTimeout = 2 };
 
 struct Args {
   const __nv_bfloat16* q;
-  const __nv_bfloat16* kv;
+  const void* kv;  // bf16 rows, or records (kQuant)
   int64_t kv_bstride;
   int64_t kv_rows;
   const int32_t* idx;
@@ -239,6 +256,60 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// One group of a producer warp's rows of a tile, as the lane's two chunks of
+// 8 dims each: chunk lane (codes) and chunk lane + 32 (codes below lane 24,
+// rotary dims from there)
+struct RecGroup {
+  uint2 lo[kGroup];
+  uint4 hi[kGroup];
+  float s_lo[kGroup], s_hi[kGroup];
+};
+
+// rows pw, pw + P, ... (the group's kGroup of them) of the tile whose indices
+// start at idx; a masked row and a row past the tile are all zero
+__device__ __forceinline__ void load_group(RecGroup& r, const uint8_t* kvb, const int32_t* idx, int row0, int lane) {
+#pragma unroll
+  for (int i = 0; i < kGroup; ++i) {
+    const int row = row0 + i * kProducerWarps;
+    const int id = row < TK ? idx[row] : -1;
+    r.lo[i] = make_uint2(0, 0);
+    r.hi[i] = make_uint4(0, 0, 0, 0);
+    r.s_lo[i] = r.s_hi[i] = 0.f;
+    if (id >= 0) {
+      const uint8_t* rec = kvb + int64_t(id) * kRecBytes;
+      const float* scales = reinterpret_cast<const float*>(rec + kNope + 2 * kRope);
+      r.lo[i] = __ldg(reinterpret_cast<const uint2*>(rec) + lane);
+      r.s_lo[i] = __ldg(scales + (lane >> 3));
+      if (lane < 24) {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(rec) + 32 + lane);
+        r.hi[i].x = w.x;
+        r.hi[i].y = w.y;
+        r.s_hi[i] = __ldg(scales + 4 + (lane >> 3));
+      } else {
+        r.hi[i] = __ldg(reinterpret_cast<const uint4*>(rec + kNope) + (lane - 24));
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void st_shared16(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+
+__device__ __forceinline__ void store_group(const RecGroup& r, uint32_t tile, int row0, int lane) {
+#pragma unroll
+  for (int i = 0; i < kGroup; ++i) {
+    const int row = row0 + i * kProducerWarps;
+    if (row < TK) {
+      st_shared16(tile + chunk_off(row, lane), kvq::bf16_values8(r.lo[i], r.s_lo[i]));
+      const uint4 h = lane < 24 ? kvq::bf16_values8(make_uint2(r.hi[i].x, r.hi[i].y), r.s_hi[i]) : r.hi[i];
+      st_shared16(tile + chunk_off(row, lane + 32), h);
+    }
+  }
+}
+
+template <bool kQuant>
 __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a,
                                                                     const __grid_constant__ CUtensorMap tm_q,
                                                                     int64_t kv_row_base_stride) {
@@ -258,7 +329,7 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a
   const int j_begin = a.lead_tiles > 0 ? a.lead_tiles * TK + split * a.rest_tps * TK : split * a.tiles_per_split * TK;
   const int j_end = max(j_begin, min(a.K, j_begin + (a.lead_tiles > 0 ? a.rest_tps : a.tiles_per_split) * TK));
   const int n = n_lead + (j_end > j_begin ? (j_end - j_begin + TK - 1) / TK : 0);
-  const bool early_lead = a.early && has_lead;
+  const bool early_lead = !kQuant && a.early && has_lead;
   const int32_t* idxr = a.idx + int64_t(mrow) * a.ld_idx;
   int32_t* s_idx = reinterpret_cast<int32_t*>(smem + kOffIdx);
 #ifdef DSA_ATTN_TRACE
@@ -275,7 +346,8 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a
     tc::mbar_init(smem_u32(&aux->q_tma), 1);
     tc::mbar_init(smem_u32(&aux->q_full), THREADS);  // every thread stores its part of Q'
     for (int s = 0; s < NT; ++s) {
-      tc::mbar_init(smem_u32(&aux->full[s]), 32 * kProducerWarps);  // one cp.async arrival per producer lane
+      // one cp.async arrival per producer lane; kQuant: one of each producer warp
+      tc::mbar_init(smem_u32(&aux->full[s]), kQuant ? kProducerWarps : 32 * kProducerWarps);
       tc::mbar_init(smem_u32(&aux->empty[s]), 2);  // both PV issuers' commits
     }
     tc::mbar_init(smem_u32(&aux->s_full), 1);
@@ -310,7 +382,8 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a
     const int j = j_begin + e - n_lead * TK;
     return j < j_end ? __ldg(idxr + j) : -1;
   };
-  const __nv_bfloat16* kvb = a.kv + int64_t(b) * kv_row_base_stride * D;
+  // (kQuant: the batch stride is in bytes and the rows are records)
+  const __nv_bfloat16* kvb = static_cast<const __nv_bfloat16*>(a.kv) + (kQuant ? 0 : int64_t(b) * kv_row_base_stride * D);
   // producers: the 16-B copies of tile t's rows pw, pw + P, ... into its slot
   auto issue_tile = [&](int t, int pw) {
     const int slot = t % NT;
@@ -397,16 +470,42 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a
     // Tiles 0 .. NT-2 are requested first; the last slot holds the query
     // block until every thread has moved its part of Q' (q_full).
     const int pw = producer_index(warp);
-    for (int t = early_lead ? 1 : 0; t < n; ++t) {
-      if (t == NT - 1) {
-        if (q_late) q_part();
-        warp_wait(&aux->q_full, 0);
+    if constexpr (kQuant) {
+      const uint8_t* recs = static_cast<const uint8_t*>(a.kv) + int64_t(b) * kv_row_base_stride;
+      RecGroup g[kGroups];
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j)
+        if (n > 0) load_group(g[j], recs, s_idx, pw + j * kGroup * kProducerWarps, lane);
+      for (int t = 0; t < n; ++t) {
+        if (t == NT - 1) {
+          if (q_late) q_part();
+          warp_wait(&aux->q_full, 0);
+        }
+        if (t >= NT) warp_wait(&aux->empty[t % NT], ((t / NT) - 1) & 1);
+        const uint32_t dst = sRing + (t % NT) * kTileBytes;
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+          const int row0 = pw + j * kGroup * kProducerWarps;
+          store_group(g[j], dst, row0, lane);
+          if (t + 1 < n) load_group(g[j], recs, s_idx + (t + 1) * TK, row0, lane);
+        }
+        tc::fence_proxy_async();  // the tile is read by the tensor cores
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(smem_u32(&aux->full[t % NT]));
       }
-      if (t >= NT) warp_wait(&aux->empty[t % NT], ((t / NT) - 1) & 1);
-      issue_tile(t, pw);
+      if (n < NT && q_late) q_part();
+    } else {
+      for (int t = early_lead ? 1 : 0; t < n; ++t) {
+        if (t == NT - 1) {
+          if (q_late) q_part();
+          warp_wait(&aux->q_full, 0);
+        }
+        if (t >= NT) warp_wait(&aux->empty[t % NT], ((t / NT) - 1) & 1);
+        issue_tile(t, pw);
+      }
+      if (n < NT && q_late) q_part();
+      cp_async_wait<0>();
     }
-    if (n < NT && q_late) q_part();
-    cp_async_wait<0>();
   } else if (warp == kMmaWarp || warp == 12) {
     // ------------------------------------------------------------ PV issuers
     // warp 4: output dims 0-255 (O^T blocks 0, 1), warp 12: dims 256-511

@@ -47,6 +47,10 @@ PROTOTYPES = {
     "dsa_linear": (I32, [P, I64, P, P, I64, I32, I32, I32, I32, I32, P, P, I32, P, I32, I32, I32, P, P]),
     "dsa_linear_packed_bytes": (ctypes.c_size_t, [I32, I32, I32]),
     "dsa_linear_pack": (I32, [P, I32, I32, I32, P, ctypes.c_size_t, P]),
+    "dsa_mxfp4_quant": (I32, [P, I32, I64, P, I64, P, P, I64, I64, P]),
+    "dsa_kv_quant_row_bytes": (SZ, [I32, I32]),
+    "dsa_kv_quant_write": (I32, [P, I64, I64, P, I64, I64, P, P, I32, I32, I32, I32, I32, I64, P]),
+    "dsa_kv_quant_read": (I32, [P, I64, I64, P, I64, P, I32, I32, I64, I32, I32, P, P]),
     "dsa_act_quant_block": (I32, [P, P, P, P, I64, I64, I64, I64, I32, F32, F32, P]),
     "dsa_kv_window_write": (I32, [P, P, P, P, I32, I32, I32, I64, I32, I32, P]),
     "dsa_kv_norm_rope_window_write": (I32, [P, I64, P, F32, P, P, I32, P, P, I64, I32, P, I64, P, I32, I32,
@@ -78,6 +82,7 @@ PROTOTYPES = {
     "dsa_sparse_attn": (I32, [P, P, I64, I64, P, I64, P, P, P, I32, I32, I32, I32, I32, F32, P, SZ, P, P]),
     "dsa_sparse_attn_ex": (I32, [P, P, I64, I64, P, I64, P, P, P, I32, I32, I32, I32, I32, F32, P, SZ, I32,
                                  ctypes.c_uint, P, P]),
+    "dsa_sparse_attn_quant": (I32, [P, P, I64, I64, P, I64, P, P, P, I32, I32, I32, I32, I32, F32, P, SZ, P, P]),
     "dsa_sparse_attn_noalloc": (I32, [P, P, I64, I64, P, I64, P, P, P, I32, I32, I32, I32, I32, F32, P, P]),
     "dsa_sparse_attn_partial": (I32, [P, P, I64, I64, P, I64, P, P, I32, I32, I32, I32, I32, F32, P, SZ, P, P]),
     "dsa_lse_combine": (I32, [P, P, P, P, I32, I32, I32, I32, P]),

@@ -210,6 +210,171 @@ def act_quant_block(x: torch.Tensor, block: int = 64, fp8_max: float = 448.0, ep
     return out, scales, codes
 
 
+_X_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _rows2d(t: torch.Tensor, name: str) -> torch.Tensor:
+    """[..., K] as a view [M, K] with unit stride in the last dim."""
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name} must have a unit stride in the last dim")
+    try:
+        t2 = t.view(-1, t.shape[-1])
+    except RuntimeError:
+        raise ValueError(f"{name} {tuple(t.shape)} with strides {t.stride()} is not a matrix of rows") from None
+    return t2
+
+
+def _ld(t2: torch.Tensor) -> int:
+    """Row stride of an [M, K] view; a single row's is never used."""
+    return t2.stride(0) if t2.shape[0] > 1 else t2.shape[1]
+
+
+def _current(t: torch.Tensor, *others) -> None:
+    """The launch goes to the current device: the tensors must be on it."""
+    for o in (t, *others):
+        if o is not None and o.device.index != torch.cuda.current_device():
+            raise ValueError(f"tensor on {o.device}, current device is cuda:{torch.cuda.current_device()}")
+
+
+def mxfp4_quant(x: torch.Tensor, out=None, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None):
+    """MXFP4 quantisation along the last dim (dsa_mxfp4_quant): blocks of 32,
+    E2M1 elements and one UE8M0 scale a block.  x [..., K] bf16, fp16 or fp32,
+    K a multiple of 32.  Returns ``(out, scales, codes)`` like
+    act_quant_block: codes [..., K/2] uint8 (the even element in the low
+    half), scales [..., K/32] uint8, and the round-trip values in x's type
+    when ``out`` is True or a tensor (which may be x), else None."""
+    _need(x, "x")
+    if x.dtype not in _X_TYPES:
+        raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
+    K = x.shape[-1] if x.dim() else 0
+    if K == 0 or K % 32:
+        raise ValueError(f"last dim {K} must be a positive multiple of 32")
+    x2 = _rows2d(x, "x")
+    M = x2.shape[0]
+    if out is True:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    o2 = None
+    if out is not None:
+        _need(out, "out", x.dtype)
+        if out.shape != x.shape:
+            raise ValueError("out must have x's shape")
+        o2 = _rows2d(out, "out")
+    if codes is None:
+        codes = torch.empty(*x.shape[:-1], K // 2, dtype=torch.uint8, device=x.device)
+    if scales is None:
+        scales = torch.empty(*x.shape[:-1], K // 32, dtype=torch.uint8, device=x.device)
+    for t, n, w in ((codes, "codes", K // 2), (scales, "scales", K // 32)):
+        _need(t, n, torch.uint8)
+        _contig(t, n)
+        if t.shape != (*x.shape[:-1], w):
+            raise ValueError(f"{n} must be {(*x.shape[:-1], w)}, got {tuple(t.shape)}")
+    _current(x, out, codes, scales)
+    if M == 0:
+        return out, scales, codes
+    check(lib().dsa_mxfp4_quant(x2.data_ptr(), _X_TYPES[x.dtype], _ld(x2), _ptr(o2), _ld(o2) if o2 is not None else 0,
+                                codes.data_ptr(), scales.data_ptr(), M, K, _stream(x)), "mxfp4_quant")
+    return out, scales, codes
+
+
+def kv_quant_row_bytes(D: int = 512, rope_dim: int = 64) -> int:
+    """Bytes of one record of the FP8 latent cache (608 for 448 + 64 dims)."""
+    n = int(lib().dsa_kv_quant_row_bytes(D, rope_dim))
+    if n == 0:
+        raise ValueError(f"D={D}, rope_dim={rope_dim}: D - rope_dim must be a positive multiple of 64, rope_dim a "
+                         "multiple of 8, D <= 8192")
+    return n
+
+
+def kv_quant_cache(B: int, rows: int, D: int = 512, rope_dim: int = 64, device=None) -> torch.Tensor:
+    """An empty FP8 latent cache [B, rows, row bytes] uint8 of zero rows."""
+    return torch.zeros(B, rows, kv_quant_row_bytes(D, rope_dim), dtype=torch.uint8,
+                       device="cuda" if device is None else device)
+
+
+def kv_quant_views(cache: torch.Tensor, D: int = 512, rope_dim: int = 64):
+    """``(codes, rope, scales)`` of a cache as views: [..., D - rope_dim]
+    float8_e4m3fn, [..., rope_dim] bf16, [..., (D - rope_dim)/64] fp32."""
+    if cache.dtype != torch.uint8 or cache.shape[-1] != kv_quant_row_bytes(D, rope_dim):
+        raise ValueError(f"cache must be uint8 with records of {kv_quant_row_bytes(D, rope_dim)} bytes")
+    a = D - rope_dim
+    b = a + 2 * rope_dim
+    return (cache[..., :a].view(torch.float8_e4m3fn), cache[..., a:b].view(BF16),
+            cache[..., b:b + a // 16].view(F32))
+
+
+def _quant_cache(cache: torch.Tensor, B: int, D: int, rope_dim: int) -> None:
+    _need(cache, "cache", torch.uint8)
+    rb = kv_quant_row_bytes(D, rope_dim)
+    if cache.dim() != 3 or cache.shape[0] < B or cache.shape[2] != rb or cache.shape[1] < 1 \
+            or cache.stride(2) != 1 or (cache.shape[1] > 1 and cache.stride(1) != rb):
+        raise ValueError(f"cache must be [>={B}, rows, {rb}] with contiguous rows (D={D}, rope_dim={rope_dim}), "
+                         f"got {tuple(cache.shape)}")
+
+
+def _per_sequence(t, name: str, B: int) -> None:
+    _need(t, name, I32)
+    _contig(t, name)
+    if t.numel() != B:
+        raise ValueError(f"{name} has {t.numel()} entries, expected {B}")
+
+
+def kv_quant_write(kv: torch.Tensor, cache: torch.Tensor, pos: torch.Tensor, win: int, offset: int = 0,
+                   rope_dim: int = 64, n_valid: torch.Tensor | None = None) -> None:
+    """Rows quantised as they are written into the FP8 latent cache
+    (dsa_kv_quant_write).  kv [B, S, D] or [B, D] bf16; cache [>=B, rows, row
+    bytes] uint8 (kv_quant_cache); pos [B] int32: token s of sequence b goes
+    to row ``offset + (pos[b] + s) % win``.  n_valid [B] int32: tokens of each
+    sequence in a padded batch.  Of more than ``win`` tokens the last ``win``
+    are written; every other row stays as it was."""
+    _need(kv, "kv", BF16)
+    if kv.dim() == 2:
+        kv = kv.unsqueeze(1)
+    if kv.dim() != 3 or kv.stride(2) != 1:
+        raise ValueError("kv must be [B, S, D] or [B, D] with a unit stride in the last dim")
+    B, S, D = kv.shape
+    _quant_cache(cache, B, D, rope_dim)
+    _per_sequence(pos, "pos", B)
+    if n_valid is not None:
+        _per_sequence(n_valid, "n_valid", B)
+    _current(kv, cache, pos, n_valid)
+    if kv.numel() == 0:
+        return
+    check(lib().dsa_kv_quant_write(kv.data_ptr(), kv.stride(0), kv.stride(1), cache.data_ptr(), cache.stride(0),
+                                   cache.shape[1], pos.data_ptr(), _ptr(n_valid), B, S, D, rope_dim, win, offset,
+                                   _stream(kv)), "kv_quant_write")
+
+
+def kv_quant_read(cache: torch.Tensor, idx: torch.Tensor | None = None, D: int = 512, rope_dim: int = 64,
+                  dtype=BF16, out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows of the FP8 latent cache back (dsa_kv_quant_read).  cache [B, rows,
+    row bytes]; idx [B, K] int32 (negative: a zero row; >= rows: clamped,
+    ``status`` bit 1) or None for every row -> [B, K, D] bf16, or fp32 (the
+    products of code and scale, not rounded) with ``dtype=torch.float32``."""
+    B = cache.shape[0]
+    _quant_cache(cache, B, D, rope_dim)
+    if dtype not in (BF16, F32):
+        raise ValueError(f"dtype must be bfloat16 or float32, got {dtype}")
+    K, ld = cache.shape[1], 0
+    if idx is not None:
+        _need(idx, "idx", I32)
+        if idx.dim() != 2 or idx.shape[0] != B or (idx.stride(1) != 1 and idx.shape[1] > 1):
+            raise ValueError(f"idx must be [{B}, K] with a unit stride in the last dim")
+        K = idx.shape[1]
+        ld = idx.stride(0) if B > 1 else K
+    if out is None:
+        out = torch.empty(B, K, D, dtype=dtype, device=cache.device)
+    _need(out, "out", dtype)
+    _contig(out, "out")
+    if tuple(out.shape) != (B, K, D):
+        raise ValueError(f"out must be {(B, K, D)}, got {tuple(out.shape)}")
+    _current(cache, idx, out, status)
+    if out.numel() == 0:
+        return out
+    check(lib().dsa_kv_quant_read(cache.data_ptr(), cache.stride(0), cache.shape[1], _ptr(idx), ld, out.data_ptr(),
+                                  int(dtype == F32), B, K, D, rope_dim, _ptr(status), _stream(cache)), "kv_quant_read")
+    return out
+
+
 def kv_window_write(kv: torch.Tensor, kv_cache: torch.Tensor, pos: torch.Tensor, win: int,
                     rope_dim: int = 64, scales: torch.Tensor | None = None) -> None:
     """act_quant on the nope dims of ``kv [B, D]`` and ring write into
@@ -718,6 +883,55 @@ def sparse_attn(q, kv, idx, sink, scale: float, out=None, lse=None, ws: Workspac
                             idx2.stride(0), sink.data_ptr(), out.data_ptr(), _ptr(lse), B, S, H, D, K, scale,
                             w.buf.data_ptr() if w else None, w.nbytes if w else 0, _ptr(status), _stream(q)),
           "sparse_attn")
+    return out
+
+
+def sparse_attn_quant(q, cache, idx, sink, scale: float, out=None, lse=None, ws: Workspace | None = None,
+                      status=None) -> torch.Tensor:
+    """``sparse_attn`` over the FP8 latent cache (dsa_sparse_attn_quant): the
+    same result as over the rows ``kv_quant_read`` returns.  q [B,S,64,512] or
+    [B,64,512] bf16; cache [>=B, rows, 608] uint8 (kv_quant_cache); idx
+    [B,S,K] / [B,K] int32, negative = masked; sink [64] fp32.  Without ``ws``
+    the scratch is allocated on the current stream for this call."""
+    _need(q, "q", BF16)
+    _contig(q, "q")
+    _need(idx, "idx", I32)
+    _need(sink, "sink", F32)
+    _contig(sink, "sink")
+    if q.dim() not in (3, 4):
+        raise ValueError("q must be [B, S, H, D] or [B, H, D]")
+    B, S, (H, D) = q.shape[0], q.shape[1] if q.dim() == 4 else 1, q.shape[-2:]
+    if (H, D) != (64, 512) or sink.numel() != H:
+        raise ValueError(f"sparse_attn_quant: built for 64 heads of 512 dims and as many sinks (got {H} of {D}, "
+                         f"{sink.numel()} sinks)")
+    _quant_cache(cache, B, D, 64)
+    K = idx.shape[-1]
+    if tuple(idx.shape[:-1]) not in ((B, S), (B,) if S == 1 else (B, S)):
+        raise ValueError(f"idx must be [B, S, K] for q {tuple(q.shape)}, got {tuple(idx.shape)}")
+    idx2 = _rows2d(idx, "idx") if idx.numel() else idx.reshape(B * S, K)
+    if out is None:
+        out = torch.empty_like(q)
+    _need(out, "out", BF16)
+    _contig(out, "out")
+    if out.shape != q.shape:
+        raise ValueError("out must have q's shape")
+    if lse is not None:
+        _need(lse, "lse", F32)
+        _contig(lse, "lse")
+        if lse.numel() != B * S * H:
+            raise ValueError(f"lse has {lse.numel()} elements, expected {B * S * H}")
+    _current(q, cache, idx, sink, out, lse, status)
+    if q.numel() == 0:
+        return out
+    L = lib()
+    need = L.dsa_sparse_attn_workspace_size(B, S, H, D, K)
+    buf = None
+    if need:
+        buf = ws.get(need) if ws is not None else torch.empty(need, dtype=torch.uint8, device=q.device)
+    check(L.dsa_sparse_attn_quant(q.data_ptr(), cache.data_ptr(), cache.stride(0), cache.shape[1],
+                                  idx2.data_ptr() if K else sink.data_ptr(), _ld(idx2), sink.data_ptr(), out.data_ptr(), _ptr(lse), B, S, H, D, K, scale,
+                                  _ptr(buf), need if buf is not None else 0, _ptr(status), _stream(q)),
+          "sparse_attn_quant")
     return out
 
 
