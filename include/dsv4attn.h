@@ -89,6 +89,37 @@ size_t dsa_linear_packed_bytes(int N, int K, int G);
  * DeviceColLinear modules are built (inference.py:4954-4966, 5934-5953). */
 int dsa_linear_pack(const void* w, int N, int K, int G, void* packed, size_t packed_bytes, dsa_stream_t stream);
 
+/* Projections over MXFP4 weights (dsa_mxfp4_quant's format):
+ *   Y[b, n] = sum_k q(X)[b, k] W[n, k],  b < B, n < N
+ * X [B, K] (x_type DSA_BF16 / DSA_FP16 / DSA_FP32, row stride ld_x) is
+ * quantised to MXFP4 in the call, the product runs on the 4-bit operands with
+ * fp32 sums; Y [B, N] (row stride ld_y) is bf16, or with out_f32 the fp32 sums
+ * themselves.  A block of X or W with a NaN scale makes its sums NaN.
+ * w_packed: W in the tile layout of dsa_linear_mxfp4_pack (16-byte aligned).
+ * K a multiple of 32; B, N, K at most 2^24; x 16-byte aligned, its row stride
+ * a multiple of 16 bytes.  workspace: dsa_linear_mxfp4_workspace_size(B, N, K)
+ * bytes (the current device's), 16-byte aligned, for X's codes and scales;
+ * calls that can overlap need their own.  status (may be NULL): bit 2 when a
+ * bounded wait ran out.
+ * The 4-bit counterpart of dsa_linear; the reference expands such weights
+ * (inference.py:283-327). */
+int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const void* w_packed, void* y, int64_t ld_y, int B,
+                     int N, int K, int out_f32, void* workspace, size_t workspace_bytes, int32_t* status,
+                     dsa_stream_t stream);
+size_t dsa_linear_mxfp4_workspace_size(int B, int N, int K);
+
+/* Bytes of the tile layout of a W [N, K] (0 for invalid sizes): ceil(N/128) x
+ * ceil(K/256) tiles of 17 KB. */
+size_t dsa_linear_mxfp4_packed_bytes(int N, int K);
+
+/* Stores a weight's codes [N, K/2] and scales [N, K/32] (both row-major,
+ * codes 16-byte aligned) once, at load time, as the tiles dsa_linear_mxfp4
+ * streams: per (128-row tile, 256-wide k-block) 16 KB of codes in the 128-byte
+ * swizzled order of the tensor cores' operand and 1 KB of scales, zero past N
+ * and K. */
+int dsa_linear_mxfp4_pack(const uint8_t* codes, const uint8_t* scales, int N, int K, void* packed,
+                          size_t packed_bytes, dsa_stream_t stream);
+
 /* ---------------------------------------------------------------- attn.kv */
 
 /* MXFP4 (OCP microscaling) quantisation of x [M, K] (row stride ld_x) along

@@ -97,3 +97,196 @@ def test_quant_refusals(cuda_dev):
         ops.mxfp4_quant(torch.zeros(2, 64, dtype=BF, device=d), codes=torch.zeros(2, 64, dtype=U8, device=d))
     with pytest.raises(ValueError, match="shape"):
         ops.mxfp4_quant(torch.zeros(2, 64, dtype=BF, device=d), out=torch.zeros(2, 32, dtype=BF, device=d))
+
+
+# --------------------------------------------------------------- projection
+
+def _w(N, K, seed):
+    """(codes, scales) of an MXFP4 weight whose rows differ in size."""
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(N, K, generator=g) * K ** -0.5 * torch.exp2(torch.randint(-4, 4, (N, 1), generator=g).float())
+    code, sc, _ = lowbit.mxfp4(w)
+    return lowbit.pack_nibbles(code), sc.to(U8)
+
+
+def _check_linear(y, x, codes, scales):
+    """Products of E2M1 values and power-of-two scales are exact; a sum of K
+    of them in fp32, in any order and with truncation, is off by at most
+    K 2^-23 of the sum of magnitudes; bf16 rounds by 2^-8."""
+    xv = lowbit.mxfp4(x)[2]
+    wv = lowbit.mxfp4_values(codes, scales)
+    exact, mag = xv @ wv.T, xv.abs() @ wv.abs().T
+    tol = mag * x.shape[1] * 2.0 ** -23 + (exact.abs() * 2.0 ** -8 if y.dtype == BF else 0.0) + 1e-30
+    err = (y.cpu().double() - exact).abs()
+    assert bool((err <= tol).all()), f"max err/tol {float((err / tol).max()):.3f}"
+
+
+SIZES = [(1, 1, 32), (1, 128, 256), (2, 7, 64), (1, 1024, 4096), (31, 200, 96), (32, 129, 288), (33, 64, 4096),
+         (64, 2048, 1024), (64, 512, 4096), (100, 2001, 512), (128, 256, 8192), (192, 384, 256), (193, 130, 544),
+         (333, 2001, 4128), (400, 64, 32), (1000, 300, 2080), (2, 24000, 1024), (700, 8200, 512), (5, 1, 8192)]
+
+
+@pytest.mark.parametrize("B,N,K", SIZES)
+@pytest.mark.parametrize("f32", [False, True])
+def test_linear_matches_the_definition(cuda_dev, B, N, K, f32):
+    from dsv4attn import ops
+    g = torch.Generator().manual_seed(B + N + K)
+    x = torch.randn(B, K, generator=g).to(BF)
+    codes, scales = _w(N, K, B * 7 + N)
+    w = ops.pack_linear_weight_mxfp4(codes.to(cuda_dev), scales.to(cuda_dev))
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_dev)
+    y = ops.linear_mxfp4(x.to(cuda_dev), w, out_f32=f32, status=status)
+    torch.cuda.synchronize()
+    assert int(status) == 0 and y.shape == (B, N) and y.dtype == (F32 if f32 else BF)
+    _check_linear(y, x, codes, scales)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_linear_input_types(cuda_dev, dtype):
+    from dsv4attn import ops
+    x = torch.randn(37, 1056, generator=torch.Generator().manual_seed(1)).to(dtype)
+    codes, scales = _w(300, 1056, 2)
+    w = ops.pack_linear_weight_mxfp4(codes.to(cuda_dev), scales.to(cuda_dev))
+    _check_linear(ops.linear_mxfp4(x.to(cuda_dev), w), x, codes, scales)
+
+
+@pytest.mark.parametrize("B", [3, 70, 250])
+@pytest.mark.parametrize("f32", [False, True])
+def test_linear_strided_rows_and_out(cuda_dev, B, f32):
+    """x a column slice, y into a wider buffer with and without 16-byte rows;
+    columns past N and the rows behind it untouched."""
+    from dsv4attn import ops
+    g = torch.Generator().manual_seed(4)
+    big = torch.randn(B, 640, generator=g).to(BF)
+    codes, scales = _w(320, 256, 3)
+    w = ops.pack_linear_weight_mxfp4(codes.to(cuda_dev), scales.to(cuda_dev))
+    xd = big.to(cuda_dev)[:, 64:320]
+    want = ops.linear_mxfp4(xd, w, out_f32=f32)
+    _check_linear(want, big[:, 64:320], codes, scales)
+    for width in (400, 403):
+        buf = torch.full((B + 1, width), 7.0, dtype=F32 if f32 else BF, device=cuda_dev)
+        got = ops.linear_mxfp4(xd, w, out=buf[:B], out_f32=f32)
+        torch.cuda.synchronize()
+        assert got.data_ptr() == buf.data_ptr() and torch.equal(buf[:B, :320], want)
+        assert bool((buf[:B, 320:] == 7.0).all()) and bool((buf[B] == 7.0).all())
+
+
+def test_linear_rows_do_not_depend_on_the_batch_around_them(cuda_dev):
+    """Rows split from a batch give the same values up to the sum's order."""
+    from dsv4attn import ops
+    x = torch.randn(290, 2048, generator=torch.Generator().manual_seed(9)).to(BF).to(cuda_dev)
+    codes, scales = _w(640, 2048, 5)
+    w = ops.pack_linear_weight_mxfp4(codes.to(cuda_dev), scales.to(cuda_dev))
+    whole = ops.linear_mxfp4(x, w, out_f32=True)
+    for n in (1, 40, 200):
+        _check_linear(ops.linear_mxfp4(x[:n], w, out_f32=True), x[:n].cpu(), codes, scales)
+    again = ops.linear_mxfp4(x, w, out_f32=True)
+    torch.cuda.synchronize()
+    assert torch.equal(whole, again)                       # a fixed order: the same bits every time
+
+
+@pytest.mark.parametrize("B", [4, 200])
+def test_linear_nan_blocks(cuda_dev, B):
+    """A NaN or an infinity in x makes its token's row NaN and no other; a NaN
+    scale in W its column."""
+    from dsv4attn import ops
+    x = torch.randn(B, 512, generator=torch.Generator().manual_seed(9)).to(BF)
+    x[1, 300] = float("nan")
+    x[3, 511] = float("inf")
+    codes, scales = _w(200, 512, 6)
+    scales[150, 3] = 255
+    w = ops.pack_linear_weight_mxfp4(codes.to(cuda_dev), scales.to(cuda_dev))
+    y = ops.linear_mxfp4(x.to(cuda_dev), w).cpu()
+    nan = torch.zeros(B, 200, dtype=torch.bool)
+    nan[[1, 3]] = True
+    nan[:, 150] = True
+    assert torch.equal(y.isnan(), nan)
+
+
+def test_linear_scale_range(cuda_dev):
+    """Weight blocks of very different size in one row, and zero rows."""
+    from dsv4attn import ops
+    x = torch.randn(20, 256, generator=torch.Generator().manual_seed(2))
+    x[:, 64:128] *= 2.0 ** 40
+    x[5] = 0
+    x = x.to(BF)
+    codes, scales = _w(130, 256, 8)
+    scales[:, 1] = 200
+    scales[:, 5] = 60
+    codes[7] = 0
+    w = ops.pack_linear_weight_mxfp4(codes.to(cuda_dev), scales.to(cuda_dev))
+    y = ops.linear_mxfp4(x.to(cuda_dev), w, out_f32=True)
+    _check_linear(y, x, codes, scales)
+    assert bool((y[5] == 0).all()) and bool((y[:, 7] == 0).all())
+
+
+def test_pack_from_floats_and_typed_views(cuda_dev):
+    from dsv4attn import ops
+    g = torch.Generator().manual_seed(3)
+    w = (torch.randn(130, 288, generator=g) * 0.1).to(BF)
+    code, sc, _ = lowbit.mxfp4(w)
+    codes, scales = lowbit.pack_nibbles(code).to(cuda_dev), sc.to(U8).to(cuda_dev)
+    a = ops.pack_linear_weight_mxfp4(codes, scales)
+    b = ops.pack_linear_weight_mxfp4(w.to(cuda_dev))
+    c = ops.pack_linear_weight_mxfp4(codes.view(torch.float4_e2m1fn_x2), scales.view(torch.float8_e8m0fnu))
+    assert a.shape == (130, 288) and torch.equal(a.packed, b.packed) and torch.equal(a.packed, c.packed)
+
+
+def test_linear_refusals(cuda_dev):
+    from dsv4attn import ops
+    d = cuda_dev
+    codes, scales = _w(64, 128, 1)
+    codes, scales = codes.to(d), scales.to(d)
+    w = ops.pack_linear_weight_mxfp4(codes, scales)
+    x = torch.zeros(4, 128, dtype=BF, device=d)
+    with pytest.raises(ValueError, match="scales"):
+        ops.pack_linear_weight_mxfp4(codes, scales[:, :3].contiguous())
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.pack_linear_weight_mxfp4(codes[:, :32], scales[:, :2].contiguous())
+    with pytest.raises(ValueError, match="without scales"):
+        ops.pack_linear_weight_mxfp4(codes)
+    with pytest.raises(ValueError, match="uint8"):
+        ops.pack_linear_weight_mxfp4(codes, scales.float())
+    with pytest.raises(TypeError, match="MXFP4Weight"):
+        ops.linear_mxfp4(x, codes)
+    with pytest.raises(ValueError, match="128"):
+        ops.linear_mxfp4(x[:, :64], w)
+    with pytest.raises(ValueError, match="bfloat16"):
+        ops.linear_mxfp4(x.double(), w)
+    with pytest.raises(ValueError, match="alignment"):
+        ops.linear_mxfp4(torch.zeros(4, 132, dtype=BF, device=d)[:, 4:], w)
+    with pytest.raises(ValueError, match="out"):
+        ops.linear_mxfp4(x, w, out=torch.zeros(3, 64, dtype=BF, device=d))
+    with pytest.raises(ValueError, match="out must be"):
+        ops.linear_mxfp4(x, w, out=torch.zeros(4, 64, dtype=F32, device=d))
+    assert ops.linear_mxfp4(x[:0], w).shape == (0, 64)
+
+
+def test_linear_captured_and_on_two_streams(cuda_dev):
+    """Two captured graphs and eager calls on a third stream, at once: each
+    keeps its own scratch."""
+    from dsv4attn import ops
+    g = torch.Generator().manual_seed(12)
+    codes, scales = _w(1024, 2048, 4)
+    w = ops.pack_linear_weight_mxfp4(codes.to(cuda_dev), scales.to(cuda_dev))
+    xs = [torch.randn(b, 2048, generator=g).to(BF).to(cuda_dev) for b in (9, 120, 300)]
+    want = [ops.linear_mxfp4(x, w) for x in xs]
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(3)]
+    for x, s in zip(xs[:2], streams):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=s):
+            outs.append(ops.linear_mxfp4(x, w))
+        graphs.append(gr)
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for gr, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                gr.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = [ops.linear_mxfp4(xs[2], w) for _ in range(4)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, wt) for o, wt in zip(outs, want))
+        assert all(torch.equal(e, want[2]) for e in eager)

@@ -154,3 +154,40 @@ def test_sparse_attn_quant_refusals():
     _refused(call(q=24), "aligned")
     _refused(call(B=32768, S=2), "65535")
     assert call(B=0) == _lib.DSA_OK
+
+
+def test_linear_mxfp4_refusals():
+    from dsv4attn import _lib
+    L = _lib.lib()
+    assert L.dsa_linear_mxfp4_packed_bytes(128, 256) == 17408
+    assert L.dsa_linear_mxfp4_packed_bytes(129, 288) == 2 * 2 * 17408
+    assert L.dsa_linear_mxfp4_packed_bytes(128, 48) == 0 and L.dsa_linear_mxfp4_packed_bytes(0, 64) == 0
+    assert L.dsa_linear_mxfp4_packed_bytes(1 << 25, 64) == 0
+    assert L.dsa_linear_mxfp4_workspace_size(0, 64, 64) == 0 and L.dsa_linear_mxfp4_workspace_size(4, 64, 48) == 0
+    # codes of 4 tokens rounded up to 256 B, scales of one k-block for one group of 128 tokens
+    assert L.dsa_linear_mxfp4_workspace_size(4, 64, 64) == 256 + 1024
+    p = L.dsa_linear_mxfp4_pack
+    _refused(p(None, 16, 128, 256, 16, 17408, None), "null")
+    _refused(p(16, 16, 128, 250, 16, 17408, None), "multiple of 32")
+    _refused(p(8, 16, 128, 256, 16, 17408, None), "aligned")
+    _refused(p(16, 16, 128, 256, 16, 17407, None), "packed buffer")
+    f = L.dsa_linear_mxfp4
+    ok = dict(x=16, xt=0, ld_x=256, w=16, y=16, ld_y=128, B=2, N=128, K=256, f32=0, ws=16, wsb=1 << 20, status=None,
+              st=None)
+
+    def call(**kw):
+        return f(*{**ok, **kw}.values())
+    _refused(call(x=None), "null")
+    _refused(call(w=None), "null")
+    _refused(call(xt=7), "x_type")
+    _refused(call(K=250), "multiple of 32")
+    _refused(call(B=-1), "B/N/K")
+    _refused(call(N=1 << 25), "2^24")
+    _refused(call(ld_x=255), "row stride")
+    _refused(call(ld_x=260), "16 bytes")
+    _refused(call(x=8), "alignment")
+    _refused(call(ld_y=127), "ld_y")
+    _refused(call(y=17), "aligned")
+    assert call(wsb=100) == _lib.DSA_ERR_WORKSPACE and "workspace" in _lib.last_error()
+    assert call(ws=None) == _lib.DSA_ERR_WORKSPACE
+    assert call(B=0) == _lib.DSA_OK

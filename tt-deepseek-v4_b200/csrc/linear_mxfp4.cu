@@ -1,0 +1,670 @@
+// Projections over MXFP4 weights on the tcgen05 tensor cores:
+//   Y[b, n] = sum_k q(X)[b, k] * W[n, k],   b < B, n < N
+// with W in MXFP4 and X quantised to MXFP4 in the call (mxfp4_dev.cuh); sums
+// in fp32, Y bf16 or fp32.  kind::mxf4 multiplies the 4-bit elements and the
+// block scales in the tensor cores: products of E2M1 values are exact and no
+// operand is expanded.
+//
+// Two launches: X's quantisation (codes [B, K/2] and block scales in the
+// order the tensor cores take them), then the product, whose weight loads
+// start before the first has ended.
+//
+// Weight layout (dsa_linear_mxfp4_pack, once at load time): per (128-row tile
+// t, 256-wide k-block kb) 17 KB: the codes of the 128 rows as a 128-byte
+// swizzled K-major operand (row r at r * 128 B, 16-byte chunk c at
+// (c ^ (r & 7)) * 16), then their 8 scales a row as two 512-byte blocks of
+// four (byte (r % 32) * 16 + (r / 32) * 4 + j), zero past N and K.  A CTA's
+// k-range is one contiguous run of memory that it reads with 17 KB bulk copies.
+//
+// A work item is (128 weight rows, Bt <= 192 tokens):
+//   warp 0      producer: per k-block the weight tile (bulk copy), the
+//               [Bt x 256] codes of X (2-D TMA) and their scales (bulk copy)
+//               into a ring;
+//   warp 1      MMA issuer: scales from shared into tensor memory
+//               (tcgen05.cp), then Y^T = W . X^T, M = 128 weight rows,
+//               N = Bt tokens, K = 64 a step, into one of two accumulators:
+//               the epilogue of item i overlaps item i + 1;
+//   warps 2-5   epilogue, thread = weight row: rounding, a staging tile
+//               [token][128] and a TMA store (element stores where Y's rows
+//               are not 16-byte aligned).
+// Tensor memory: 2 x 192 accumulator columns and 2 x 24 of scales (8 for W, 16
+// for X a k-block).
+//
+// Few items (decode): the C CTAs of a cluster share an item, each over its
+// own part of K.  After the last product a cluster barrier frees every ring;
+// each CTA writes its partial [Bt][128] there, copies each owner's rows to it
+// through distributed shared memory, and the owner sums the C partials in rank
+// order: the same sum on every run.
+#include "cluster.cuh"
+#include "common.cuh"
+#include "mxfp4_dev.cuh"
+#include "tc05.cuh"
+#include "tma.cuh"
+
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+#include <type_traits>
+
+namespace dsa {
+namespace lmx {
+
+constexpr int TILE_N = 128;
+constexpr int KBW = 256;                        // k a stage: 128 B of codes a row
+constexpr int kSfPerKb = KBW / mx::kBlock;      // 8 scales
+constexpr int kCodeBytes = TILE_N * KBW / 2;    // 16 KB
+constexpr int kSfBytes = TILE_N * kSfPerKb;     // 1 KB for each 128 rows
+constexpr int kWBytes = kCodeBytes + kSfBytes;  // a weight tile
+constexpr int kMaxBt = 192;
+constexpr int kMaxStages = 12;
+constexpr int kMaxSplit = 16;
+constexpr int THREADS = 192;
+constexpr int kSmemBytes = 232448;
+constexpr int kAuxBytes = 256;
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColSf = 2 * kMaxBt;         // scales: per parity 8 columns of W, 16 of X
+constexpr uint32_t kSfCols = 24;
+static_assert(kColSf + 2 * kSfCols <= kTmemCols, "TMEM columns");
+static_assert(kWBytes % 1024 == 0, "the swizzled operands start on 1024 B");
+
+struct Args {
+  const uint8_t* w;
+  const uint8_t* xsf;   // X's scales: [m tile][k-block][groups of 128 tokens] of 1 KB
+  void* y;
+  int64_t ld_y;
+  int B, Bt, groups, N, nkb, n_tiles, m_tiles;
+  int split, rows_per;  // C CTAs an item; token rows each of them finishes
+  int n_stages, tma_store;
+  uint32_t stage_bytes, part_off, recv_off, out_off, aux_off;
+  int32_t* status;
+  long long wait_limit;
+};
+
+struct Aux {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint64_t ready;
+  uint32_t tmem_base;
+};
+static_assert(sizeof(Aux) <= kAuxBytes, "aux block");
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(x), "r"(y)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+template <bool kF32>
+using OutT = typename std::conditional<kF32, float, __nv_bfloat16>::type;
+template <bool kF32>
+__device__ __forceinline__ OutT<kF32> to_out(float v) {
+  if constexpr (kF32) return v;
+  else return f2bf(v);
+}
+
+// CNT values of token rows [row, row + CNT) of the item's tile: staged at rows
+// [srow, ..) or stored to Y; rows from `rows` on are left out
+template <bool kF32, int CNT>
+__device__ __forceinline__ void put_rows(const Args& a, OutT<kF32>* stage, int srow, int nr, int64_t row, int rows,
+                                         int n, const float* v) {
+  if (a.tma_store) {
+#pragma unroll
+    for (int i = 0; i < CNT; ++i)
+      if (i < rows) stage[(srow + i) * TILE_N + nr] = to_out<kF32>(v[i]);
+  } else if (n < a.N) {
+    OutT<kF32>* o = static_cast<OutT<kF32>*>(a.y) + row * a.ld_y + n;
+#pragma unroll
+    for (int i = 0; i < CNT; ++i)
+      if (i < rows) o[i * a.ld_y] = to_out<kF32>(v[i]);
+  }
+}
+
+template <bool kF32>
+__global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
+                                                                  const __grid_constant__ CUtensorMap tm_x,
+                                                                  const __grid_constant__ CUtensorMap tm_y) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Aux* aux = reinterpret_cast<Aux*>(smem + a.aux_off);
+  const uint32_t sbase = smem_u32(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int C = a.split;
+  const int rank = C > 1 ? int(lin::cluster_rank()) : 0;
+  const int cid = blockIdx.x / C, n_cl = gridDim.x / C;
+  const int n_items = a.n_tiles * a.m_tiles;
+  const int kb0 = rank * a.nkb / C, kb1 = (rank + 1) * a.nkb / C;
+  const int NS = a.n_stages;
+  const uint32_t x_bytes = uint32_t(a.Bt) * (KBW / 2), xsf_bytes = uint32_t(a.groups) * kSfBytes;
+  const uint32_t stage_tx = kWBytes + x_bytes + xsf_bytes;
+
+  if (warp == 1) {
+    tc::tmem_alloc(smem_u32(&aux->tmem_base), kTmemCols);
+    tc::tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      tc::mbar_init(smem_u32(&aux->full[s]), 1);
+      tc::mbar_init(smem_u32(&aux->empty[s]), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      tc::mbar_init(smem_u32(&aux->acc_full[s]), 1);
+      tc::mbar_init(smem_u32(&aux->acc_empty[s]), 4);
+    }
+    tc::mbar_init(smem_u32(&aux->ready), 1);  // the owner's arrival + the copied bytes
+    tc::mbar_fence_init();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = aux->tmem_base;
+
+  // the weights come from no kernel of this call: their first tiles are
+  // requested before the dependency wait, X's codes and scales after it
+  int npre = 0;
+  if (warp == 0 && lane == 0) {
+    for (int item = cid; item < n_items && npre < NS; item += n_cl) {
+      const uint8_t* wt = a.w + (int64_t(item / a.m_tiles) * a.nkb + kb0) * kWBytes;
+      for (int kb = kb0; kb < kb1 && npre < NS; ++kb, ++npre, wt += kWBytes) {
+        const uint32_t fb = smem_u32(&aux->full[npre]);
+        tma::mbar_arrive_expect_tx(fb, stage_tx);
+        lin::bulk_load(sbase + npre * a.stage_bytes, wt, kWBytes, fb);
+      }
+    }
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer
+    if (lane == 0) {
+      tma::prefetch_map(&tm_x);
+      int it = 0;
+      for (int item = cid; item < n_items; item += n_cl) {
+        const int t = item / a.m_tiles, mt = item - t * a.m_tiles;
+        const uint8_t* wt = a.w + (int64_t(t) * a.nkb + kb0) * kWBytes;
+        const uint8_t* xs = a.xsf + (int64_t(mt) * a.nkb + kb0) * xsf_bytes;
+        for (int kb = kb0; kb < kb1; ++kb, ++it, wt += kWBytes, xs += xsf_bytes) {
+          const int s = it % NS;
+          const uint32_t st = sbase + s * a.stage_bytes;
+          const uint32_t fb = smem_u32(&aux->full[s]);
+          if (it >= npre) {
+            if (it >= NS) tc::mbar_wait(smem_u32(&aux->empty[s]), ((it / NS) - 1) & 1, a.status, 2, a.wait_limit);
+            tma::mbar_arrive_expect_tx(fb, stage_tx);
+            lin::bulk_load(st, wt, kWBytes, fb);
+          }
+          // (the map's columns are pairs of codes: 64 two-byte words a k-block)
+          tma::load_2d(st + kWBytes, &tm_x, kb * (KBW / 4), mt * a.Bt, fb);
+          lin::bulk_load(st + kWBytes + x_bytes, xs, xsf_bytes, fb);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      const uint32_t id0 = tc::idesc_mxf4(128, a.Bt, 0), id2 = tc::idesc_mxf4(128, a.Bt, 2);
+      int it = 0, li = 0;
+      for (int item = cid; item < n_items; item += n_cl, ++li) {
+        const int acc = li & 1;
+        if (li >= 2) tc::mbar_wait(smem_u32(&aux->acc_empty[acc]), ((li - 2) >> 1) & 1, a.status, 2, a.wait_limit);
+        tc::fence_after_sync();
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int s = it % NS;
+          tc::mbar_wait(smem_u32(&aux->full[s]), (it / NS) & 1, a.status, 2, a.wait_limit);
+          tc::fence_after_sync();
+          const uint32_t st = sbase + s * a.stage_bytes;
+          const uint32_t sx = st + kWBytes + x_bytes;
+          const uint32_t sfa = tmem + kColSf + kSfCols * (it & 1), sfb = sfa + 8;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            tc::cp_scales(sfa + 4 * j, st + kCodeBytes + 512 * j);
+            for (int g = 0; g < a.groups; ++g) tc::cp_scales(sfb + 8 * j + 4 * g, sx + g * kSfBytes + 512 * j);
+          }
+#pragma unroll
+          for (int ks = 0; ks < KBW / 64; ++ks) {
+            const uint64_t ad = tc::smem_desc(st + ks * 32, 16, 1024, tc::kLayoutSw128);
+            const uint64_t bd = tc::smem_desc(st + kWBytes + ks * 32, 16, 1024, tc::kLayoutSw128);
+            tc::mma_mxf4(tmem + uint32_t(kMaxBt) * acc, ad, bd, (ks & 1) ? id2 : id0, sfa + 4 * (ks >> 1),
+                         sfb + 8 * (ks >> 1), (kb > kb0 || ks) ? 1u : 0u);
+          }
+          tc::mma_commit(smem_u32(&aux->empty[s]));
+        }
+        tc::mma_commit(smem_u32(&aux->acc_full[acc]));
+      }
+    }
+    __syncwarp();
+  }
+
+  if (warp >= 2) {
+    // ---------------------------------------------------------------- epilogue (warps 2-5)
+    const int quarter = warp & 3;        // TMEM lanes [32 quarter, 32 quarter + 32)
+    const int nr = quarter * 32 + lane;  // this thread's row of the weight tile
+    const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16);
+    OutT<kF32>* stage = reinterpret_cast<OutT<kF32>*>(smem + a.out_off);
+    const bool lead = tid == 64;
+    if (lead && a.tma_store) tma::prefetch_map(&tm_y);
+    if (C == 1) {
+      int li = 0;
+      for (int item = cid; item < n_items; item += n_cl, ++li) {
+        const int acc = li & 1;
+        const int t = item / a.m_tiles, mt = item - t * a.m_tiles;
+        const int64_t b0 = int64_t(mt) * a.Bt;
+        const int rows = int(min(int64_t(a.Bt), a.B - b0));
+        if (a.tma_store && li > 0) {  // the tile before has left the staging buffer
+          if (lead) lin::bulk_wait_read();
+          tc::named_bar_sync(1, 128);
+        }
+        tc::mbar_wait(smem_u32(&aux->acc_full[acc]), (li >> 1) & 1, a.status, 2, a.wait_limit);
+        tc::fence_after_sync();
+        for (int c0 = 0; c0 < rows; c0 += 32) {
+          float v[32];
+          tc::tmem_ld32(trow + uint32_t(kMaxBt) * acc + c0, v);
+          tc::tmem_wait_ld();
+          put_rows<kF32, 32>(a, stage, c0, nr, b0 + c0, rows - c0, t * TILE_N + nr, v);
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(smem_u32(&aux->acc_empty[acc]));
+        if (a.tma_store) {
+          tc::fence_proxy_async();
+          tc::named_bar_sync(1, 128);
+          if (lead) tma_store_2d(&tm_y, smem_u32(stage), t * TILE_N, int(b0));
+        }
+      }
+    } else {
+      tc::mbar_wait(smem_u32(&aux->acc_full[0]), 0, a.status, 2, a.wait_limit);
+      tc::fence_after_sync();
+    }
+    if (C > 1) {
+      // one item a cluster; every CTA's products are done once all have arrived
+      lin::cluster_arrive();
+      lin::cluster_wait();
+      const int t = cid / a.m_tiles, mt = cid - t * a.m_tiles;
+      const int64_t b0 = int64_t(mt) * a.Bt;
+      const int rows = int(min(int64_t(a.Bt), a.B - b0));
+      const int R = a.rows_per, r0 = rank * R, own = max(0, min(rows, r0 + R) - r0);
+      float* part = reinterpret_cast<float*>(smem + a.part_off);
+      const float* recv = reinterpret_cast<const float*>(smem + a.recv_off);
+      for (int c0 = 0; c0 < rows; c0 += 32) {
+        float v[32];
+        tc::tmem_ld32(trow + c0, v);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (c0 + i < rows) part[(c0 + i) * TILE_N + nr] = v[i];
+      }
+      tc::fence_proxy_async();  // the copy engine reads the partial
+      tc::named_bar_sync(1, 128);
+      if (lead) {
+        tma::mbar_arrive_expect_tx(smem_u32(&aux->ready), uint32_t(C * own) * TILE_N * 4u);
+        for (int q = 0; q < C; ++q) {
+          const int n = min(R, rows - q * R);
+          if (n <= 0) break;
+          lin::bulk_to_peer(lin::mapa(smem_u32(recv) + uint32_t(rank * R) * TILE_N * 4u, q),
+                            smem_u32(part) + uint32_t(q * R) * TILE_N * 4u, uint32_t(n) * TILE_N * 4u,
+                            lin::mapa(smem_u32(&aux->ready), q));
+        }
+      }
+      lin::mbar_wait_cluster(smem_u32(&aux->ready), 0, a.status, a.wait_limit);
+      for (int l0 = 0; l0 < own; l0 += 8) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+        for (int q = 0; q < C; ++q) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] += recv[(q * R + min(l0 + j, R - 1)) * TILE_N + nr];
+        }
+        put_rows<kF32, 8>(a, stage, l0, nr, b0 + r0 + l0, own - l0, t * TILE_N + nr, v);
+      }
+      if (a.tma_store && own > 0) {
+        tc::fence_proxy_async();
+        tc::named_bar_sync(1, 128);
+        if (lead) tma_store_2d(&tm_y, smem_u32(stage), t * TILE_N, int(b0) + r0);
+      }
+    }
+    if (lead) lin::bulk_wait_read();  // the tiles have left shared memory
+  } else if (C > 1) {
+    lin::cluster_arrive();
+    lin::cluster_wait();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (C > 1) {  // no CTA leaves while a peer may still touch its shared memory
+    lin::cluster_arrive();
+    lin::cluster_wait();
+  }
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// X [B, K] -> codes [B, K/2] and scales in the product's order; the scales of
+// the last k-block past K are zero (their codes are zero-filled by the TMA).
+constexpr int kQuantThreads = 256;
+constexpr int kQuantUnroll = 2;
+template <typename T>
+__global__ void __launch_bounds__(kQuantThreads) quant_x_kernel(const T* __restrict__ x, int64_t ld_x,
+                                                                uint32_t* __restrict__ codes,
+                                                                uint8_t* __restrict__ sf, int64_t total, int row_chunks,
+                                                                int Bt, int groups, int nkb) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t step = int64_t(gridDim.x) * kQuantThreads * kQuantUnroll;
+  for (int64_t c0 = int64_t(blockIdx.x) * kQuantThreads * kQuantUnroll; c0 < total; c0 += step) {
+    float v[kQuantUnroll][mx::kVec];
+    int64_t at[kQuantUnroll];
+    int row[kQuantUnroll], col[kQuantUnroll];
+#pragma unroll
+    for (int u = 0; u < kQuantUnroll; ++u) {
+      at[u] = c0 + u * kQuantThreads + threadIdx.x;
+      row[u] = col[u] = 0;
+#pragma unroll
+      for (int i = 0; i < mx::kVec; ++i) v[u][i] = 0.f;
+      if (at[u] < total) {
+        row[u] = int(at[u] / row_chunks);
+        col[u] = int(at[u] - int64_t(row[u]) * row_chunks);
+        mx::load8(x + row[u] * ld_x + int64_t(col[u]) * mx::kVec, v[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kQuantUnroll; ++u) {
+      const uint32_t sc = mx::scale_code(v[u]);
+      if (at[u] >= total) continue;
+      codes[at[u]] = mx::codes8(v[u], sc);
+      if ((col[u] & 3) == 0) {
+        const int mt = row[u] / Bt, r = row[u] - mt * Bt;
+        int i = col[u] >> 2;  // the block's number along K
+        const bool last = col[u] + 4 == row_chunks;
+        do {
+          const int kb = i / kSfPerKb, j = i % kSfPerKb;
+          sf[((int64_t(mt) * nkb + kb) * groups + (r >> 7)) * kSfBytes + (j >> 2) * 512 + (r & 31) * 16 +
+             ((r >> 5) & 3) * 4 + (j & 3)] = uint8_t(i == (col[u] >> 2) ? sc : 0u);
+          ++i;
+        } while (last && i < nkb * kSfPerKb);
+      }
+    }
+  }
+}
+
+// codes [N, K/2], scales [N, K/32] row-major -> the weight tiles, 16 B a thread
+__global__ void pack_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                            uint8_t* __restrict__ out, int N, int K, int nkb, int64_t chunks) {
+  constexpr int kChunks = kWBytes / 16;  // of a tile
+  for (int64_t id = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; id < chunks; id += int64_t(gridDim.x) * blockDim.x) {
+    const int64_t tile = id / kChunks;
+    const int within = int(id - tile * kChunks);
+    const int kb = int(tile % nkb), t = int(tile / nkb);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    uint8_t* dst = out + tile * kWBytes;
+    if (within < kCodeBytes / 16) {
+      const int r = within >> 3, c = within & 7;
+      const int n = t * TILE_N + r, k = kb * KBW + c * 32;
+      if (n < N && k < K) v = *reinterpret_cast<const uint4*>(codes + int64_t(n) * (K / 2) + k / 2);
+      dst += r * 128 + ((c ^ (r & 7)) << 4);
+    } else {
+      // 16 B of scales: rows r, r + 32, r + 64, r + 96, four scales each
+      const int s = within - kCodeBytes / 16, half = s >> 5, r = s & 31;
+      uint8_t* b = reinterpret_cast<uint8_t*>(&v);
+      for (int q = 0; q < 4; ++q) {
+        const int n = t * TILE_N + q * 32 + r;
+        for (int j = 0; j < 4; ++j) {
+          const int i = kb * kSfPerKb + half * 4 + j;
+          if (n < N && i < K / mx::kBlock) b[q * 4 + j] = scales[int64_t(n) * (K / mx::kBlock) + i];
+        }
+      }
+      dst += kCodeBytes + s * 16;
+    }
+    *reinterpret_cast<uint4*>(dst) = v;
+  }
+}
+
+// Clusters of C CTAs that can be resident at once (one CTA per SM), C = 1 ..
+// kMaxSplit, for the current device; NULL without one.  Filled at its first
+// call on a device, which also raises the kernels' shared-memory limit.
+static const int* cluster_table() {
+  static int table[64][kMaxSplit + 1];
+  static std::once_flag once[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  std::call_once(once[dev], [dev] {
+    int* n = table[dev];
+    for (auto k : {linear_mxfp4_kernel<false>, linear_mxfp4_kernel<true>}) {
+      if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) != cudaSuccess ||
+          cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+        cudaGetLastError();
+        return;
+      }
+    }
+    n[1] = num_sms();
+    for (int C = 2; C <= kMaxSplit; ++C) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(C);
+      cfg.blockDim = dim3(THREADS);
+      cfg.dynamicSmemBytes = kSmemBytes;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = C;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&n[C], linear_mxfp4_kernel<false>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n[C] = 0;
+      }
+    }
+  });
+  return table[dev][1] > 0 ? table[dev] : nullptr;
+}
+
+struct Plan {
+  int Bt, m_tiles, groups, split;
+};
+
+// shared memory of a plan: the ring's stages (0: it does not fit) and offsets
+static int lay_out(const Plan& p, int B, int es, bool tma_store, Args* a) {
+  const int tokens = std::min(B, p.Bt);
+  const int R = (tokens + p.split - 1) / p.split;
+  const int out_rows = p.split > 1 ? R : p.Bt;
+  const uint32_t stage = uint32_t(kWBytes + p.Bt * (KBW / 2) + p.groups * kSfBytes);
+  const uint32_t out_bytes = tma_store ? (uint32_t(out_rows) * TILE_N * es + 1023u) & ~1023u : 0u;
+  const uint32_t part = p.split > 1 ? uint32_t(tokens) * TILE_N * 4 : 0u;
+  const uint32_t recv = p.split > 1 ? uint32_t(p.split * R) * TILE_N * 4 : 0u;
+  const uint32_t room = kSmemBytes - 1024 - kAuxBytes;
+  if (out_bytes >= room || part + recv + out_bytes > room) return 0;
+  const int stages = std::min<int>(kMaxStages, (room - out_bytes) / stage);
+  if (stages < 2) return 0;
+  const uint32_t ring = std::max(stages * stage, part + recv);  // the partials take the ring's place
+  if (a) {
+    a->n_stages = stages;
+    a->stage_bytes = stage;
+    a->rows_per = R;
+    a->part_off = 0;
+    a->recv_off = part;
+    a->out_off = ring;
+    a->aux_off = ring + out_bytes;
+  }
+  return stages;
+}
+
+// Tokens an item and CTAs an item: the pair with the lowest estimate of the
+// busiest CTA's cycles.  A k-block costs what its bytes take to reach the SM
+// (~48 B a cycle) and at least its four MMAs (~90 cycles each, 2 Bt at full
+// rate); an item costs a fixed ~2K cycles and its share of the epilogue, a
+// split ~3K more and the exchange of its partials.
+static Plan pick_plan(int B, int N, int nkb) {
+  static const int kNone[kMaxSplit + 1] = {0, 148};  // no device: unsplit
+  const int* clusters = cluster_table();
+  if (!clusters) clusters = kNone;
+  const int n_tiles = (N + TILE_N - 1) / TILE_N;
+  Plan best{0, 0, 0, 0};
+  double best_cost = 0;
+  for (int want : {32, 48, 64, 96, 128, 160, 192}) {
+    const int m_tiles = (B + want - 1) / want;
+    const int Bt = std::max(32, ((B + m_tiles - 1) / m_tiles + 15) / 16 * 16);
+    const int64_t items = int64_t(n_tiles) * m_tiles;
+    const double kb_cost = std::max((kWBytes + Bt * 136.0) / 48.0, std::max(360.0, 2.0 * Bt));
+    for (int C = 1; C <= std::min(kMaxSplit, nkb); ++C) {
+      if (C > 1 && items > clusters[C]) continue;
+      Plan p{Bt, m_tiles, (Bt + 127) / 128, C};
+      if (!lay_out(p, B, 4, true, nullptr)) continue;
+      const int64_t waves = C > 1 ? 1 : (items + clusters[1] - 1) / clusters[1];
+      const double cost = waves * ((nkb + C - 1) / C * kb_cost + 1500) + Bt * 8.0 + 2000 + (C > 1 ? 3000 + Bt * 16.0 : 0);
+      if (best.Bt == 0 || cost < best_cost) {
+        best_cost = cost;
+        best = p;
+      }
+    }
+  }
+  return best;
+}
+
+static int64_t code_bytes(int64_t B, int64_t K) { return (B * (K / 2) + 255) / 256 * 256; }
+static int n_kblocks(int K) { return (K + KBW - 1) / KBW; }
+static bool good_sizes(int64_t B, int64_t N, int64_t K) {
+  return B >= 0 && B <= (1 << 24) && N > 0 && N <= (1 << 24) && K > 0 && K <= (1 << 24) && K % mx::kBlock == 0;
+}
+
+}  // namespace lmx
+}  // namespace dsa
+
+using namespace dsa;
+
+extern "C" size_t dsa_linear_mxfp4_packed_bytes(int N, int K) {
+  if (!lmx::good_sizes(0, N, K)) return 0;
+  return size_t((N + lmx::TILE_N - 1) / lmx::TILE_N) * lmx::n_kblocks(K) * lmx::kWBytes;
+}
+
+extern "C" int dsa_linear_mxfp4_pack(const uint8_t* codes, const uint8_t* scales, int N, int K, void* packed,
+                                     size_t packed_bytes, dsa_stream_t stream) {
+  clear_error();
+  DSA_CHECK_ARG(codes && scales && packed, "linear_mxfp4_pack: null codes/scales/packed");
+  DSA_CHECK_ARG(lmx::good_sizes(0, N, K), "linear_mxfp4_pack: bad N/K (K a multiple of 32, at most 2^24)");
+  DSA_CHECK_ARG(aligned(codes, 16) && aligned(packed, 16), "linear_mxfp4_pack: codes/packed must be 16-byte aligned");
+  const size_t need = dsa_linear_mxfp4_packed_bytes(N, K);
+  DSA_CHECK_ARG(packed_bytes >= need, "linear_mxfp4_pack: packed buffer %zu bytes < %zu", packed_bytes, need);
+  const int64_t chunks = int64_t(need / 16);
+  const int grid = int(std::min<int64_t>((chunks + 255) / 256, int64_t(num_sms()) * 16));
+  lmx::pack_kernel<<<grid, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      codes, scales, static_cast<uint8_t*>(packed), N, K, lmx::n_kblocks(K), chunks);
+  DSA_CHECK_LAUNCH("linear_mxfp4_pack");
+  return DSA_OK;
+}
+
+extern "C" size_t dsa_linear_mxfp4_workspace_size(int B, int N, int K) {
+  if (!lmx::good_sizes(B, N, K) || B == 0) return 0;
+  const int nkb = lmx::n_kblocks(K);
+  const lmx::Plan p = lmx::pick_plan(B, N, nkb);
+  return size_t(lmx::code_bytes(B, K)) + size_t(p.m_tiles) * nkb * p.groups * lmx::kSfBytes;
+}
+
+extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const void* w_packed, void* y, int64_t ld_y,
+                                int B, int N, int K, int out_f32, void* workspace, size_t workspace_bytes,
+                                int32_t* status, dsa_stream_t stream) {
+  clear_error();
+  DSA_CHECK_ARG(x && w_packed && y, "linear_mxfp4: null x/w/y");
+  DSA_CHECK_ARG(x_type == DSA_BF16 || x_type == DSA_FP16 || x_type == DSA_FP32, "linear_mxfp4: unknown x_type %d",
+                x_type);
+  DSA_CHECK_ARG(lmx::good_sizes(B, N, K), "linear_mxfp4: bad B/N/K (K a multiple of 32, each at most 2^24)");
+  const int xs = x_type == DSA_FP32 ? 4 : 2, es = out_f32 ? 4 : 2;
+  DSA_CHECK_ARG(aligned(x, 16) && aligned(w_packed, 16) && (B <= 1 || (ld_x >= K && ld_x * xs % 16 == 0)),
+                "linear_mxfp4: x needs 16-byte alignment and a row stride >= K, a multiple of 16 bytes");
+  DSA_CHECK_ARG((B <= 1 || ld_y >= N) && aligned(y, es), "linear_mxfp4: ld_y < N, or y not aligned to its type");
+  if (B == 0) return DSA_OK;
+  const int nkb = lmx::n_kblocks(K);
+  const lmx::Plan p = lmx::pick_plan(B, N, nkb);
+  const int64_t cb = lmx::code_bytes(B, K);
+  const size_t need = size_t(cb) + size_t(p.m_tiles) * nkb * p.groups * lmx::kSfBytes;
+  if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)) {
+    set_error("linear_mxfp4: needs %zu bytes of 16-byte aligned workspace (got %zu)", need, workspace_bytes);
+    return DSA_ERR_WORKSPACE;
+  }
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  uint8_t* sf = codes + cb;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+
+  lmx::Args a{};
+  a.w = static_cast<const uint8_t*>(w_packed);
+  a.xsf = sf;
+  a.y = y;
+  a.ld_y = ld_y;
+  a.B = B;
+  a.Bt = p.Bt;
+  a.groups = p.groups;
+  a.N = N;
+  a.nkb = nkb;
+  a.n_tiles = (N + lmx::TILE_N - 1) / lmx::TILE_N;
+  a.m_tiles = p.m_tiles;
+  a.split = p.split;
+  a.tma_store = aligned(y, 16) && (B == 1 || ld_y * es % 16 == 0) && int64_t(N) * es % 16 == 0 ? 1 : 0;
+  // a split's last owner may hold fewer rows than its box: below the last
+  // token tile the box would reach into the next one
+  if (p.split > 1 && p.m_tiles > 1 && p.Bt % p.split != 0) a.tma_store = 0;
+  a.status = status;
+  a.wait_limit = wait_limit_cycles();
+  if (!lmx::cluster_table() || !lmx::lay_out(p, B, es, a.tma_store, &a)) {
+    set_error("linear_mxfp4: no launch configuration fits");
+    return DSA_ERR_CUDA;
+  }
+  CUtensorMap tm_x, tm_y;
+  memset(&tm_y, 0, sizeof(tm_y));
+  // codes as [B, K/4] two-byte words
+  if (!tma::make_2d_bf16(&tm_x, codes, uint64_t(K) / 4, uint64_t(B), uint64_t(K) / 2, 64, uint32_t(p.Bt))) {
+    set_error("linear_mxfp4: cuTensorMapEncodeTiled failed");
+    return DSA_ERR_CUDA;
+  }
+  if (a.tma_store) {
+    tma::EncodeTiledFn fn = tma::encode_fn();
+    const cuuint64_t dims[2] = {uint64_t(N), uint64_t(B)};
+    const cuuint64_t strides[1] = {uint64_t(B == 1 ? N : ld_y) * es};
+    const cuuint32_t box[2] = {uint32_t(lmx::TILE_N), uint32_t(p.split > 1 ? a.rows_per : p.Bt)};
+    const cuuint32_t estr[2] = {1, 1};
+    if (!fn || fn(&tm_y, out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, y, dims,
+                  strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+      set_error("linear_mxfp4: cuTensorMapEncodeTiled (Y) failed");
+      return DSA_ERR_CUDA;
+    }
+  }
+  const int64_t total = int64_t(B) * (K / mx::kVec);
+  const int per = lmx::kQuantThreads * lmx::kQuantUnroll;
+  const dim3 qgrid(unsigned(std::min<int64_t>((total + per - 1) / per, int64_t(num_sms()) * 16)));
+  auto quant = [&](auto* ptr) {
+    using T = std::remove_pointer_t<decltype(ptr)>;
+    launch_pdl(lmx::quant_x_kernel<T>, qgrid, dim3(lmx::kQuantThreads), 0, st, static_cast<const T*>(x), ld_x,
+               reinterpret_cast<uint32_t*>(codes), sf, total, K / mx::kVec, p.Bt, p.groups, nkb);
+  };
+  if (x_type == DSA_BF16)
+    quant(static_cast<__nv_bfloat16*>(nullptr));
+  else if (x_type == DSA_FP16)
+    quant(static_cast<__half*>(nullptr));
+  else
+    quant(static_cast<float*>(nullptr));
+  DSA_CHECK_LAUNCH("linear_mxfp4 (quantisation)");
+  const int64_t items = int64_t(a.n_tiles) * a.m_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(p.split > 1 ? items * p.split : std::min<int64_t>(items, num_sms())));
+  cfg.blockDim = dim3(lmx::THREADS);
+  cfg.dynamicSmemBytes = lmx::kSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.split > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, out_f32 ? lmx::linear_mxfp4_kernel<true> : lmx::linear_mxfp4_kernel<false>, a, tm_x, tm_y);
+  DSA_CHECK_LAUNCH("linear_mxfp4");
+  return DSA_OK;
+}

@@ -82,6 +82,33 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate));
 }
 
+// Block-scaled MXFP4 (kind::mxf4): E2M1 operands, 64 a step, one UE8M0 scale
+// for each 32 in tensor memory.  Instruction descriptor: scale id of B bits
+// 4-5, A format 7-9 and B format 10-12 (1 = E2M1), N>>3 bits 17-22, scale
+// type bit 23 (1 = UE8M0), M>>4 bits 24-28, scale id of A bits 29-30.  A
+// 32-bit column of tensor memory holds four scales of a row: scale id 0 takes
+// bytes 0-1, scale id 2 bytes 2-3.
+__host__ __device__ constexpr uint32_t idesc_mxf4(int M, int N, int sf_id) {
+  return ((uint32_t)sf_id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) |
+         ((uint32_t)(M >> 4) << 24) | ((uint32_t)sf_id << 29);
+}
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(
+          d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate));
+}
+// 32 rows of 16 B in shared memory (8x16-B core matrices, 128 B apart) into
+// four columns of tensor memory, the same for each of the four 32-lane
+// sub-partitions; ordered before the tcgen05.mma this thread issues next
+__device__ __forceinline__ void cp_scales(uint32_t tmem, uint32_t saddr) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem),
+               "l"(smem_desc(saddr, 16, 128, kLayoutNone)));
+}
+
 // arrive on an mbarrier once all previously issued tcgen05.mma of this thread complete
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)

@@ -47,6 +47,10 @@ PROTOTYPES = {
     "dsa_linear": (I32, [P, I64, P, P, I64, I32, I32, I32, I32, I32, P, P, I32, P, I32, I32, I32, P, P]),
     "dsa_linear_packed_bytes": (ctypes.c_size_t, [I32, I32, I32]),
     "dsa_linear_pack": (I32, [P, I32, I32, I32, P, ctypes.c_size_t, P]),
+    "dsa_linear_mxfp4": (I32, [P, I32, I64, P, P, I64, I32, I32, I32, I32, P, SZ, P, P]),
+    "dsa_linear_mxfp4_workspace_size": (SZ, [I32, I32, I32]),
+    "dsa_linear_mxfp4_packed_bytes": (SZ, [I32, I32]),
+    "dsa_linear_mxfp4_pack": (I32, [P, P, I32, I32, P, SZ, P]),
     "dsa_mxfp4_quant": (I32, [P, I32, I64, P, I64, P, P, I64, I64, P]),
     "dsa_kv_quant_row_bytes": (SZ, [I32, I32]),
     "dsa_kv_quant_write": (I32, [P, I64, I64, P, I64, I64, P, P, I32, I32, I32, I32, I32, I64, P]),

@@ -181,6 +181,93 @@ def linear(x: torch.Tensor, w, out: torch.Tensor | None = None, groups: int = 1,
     return out
 
 
+class MXFP4Weight:
+    """An MXFP4 projection weight W [N, K] stored once in the tile layout the
+    kernel streams (dsa_linear_mxfp4_pack): ``packed`` is a uint8 device
+    tensor, 17/32 of a byte an element (rows and K rounded up to tiles of 128
+    x 256)."""
+
+    __slots__ = ("packed", "N", "K")
+
+    def __init__(self, packed: torch.Tensor, N: int, K: int):
+        self.packed, self.N, self.K = packed, N, K
+
+    @property
+    def device(self):
+        return self.packed.device
+
+    @property
+    def shape(self):
+        return (self.N, self.K)
+
+
+def pack_linear_weight_mxfp4(codes: torch.Tensor, scales: torch.Tensor | None = None) -> MXFP4Weight:
+    """An MXFP4 checkpoint weight -> MXFP4Weight: codes [N, K/2] (uint8, int8
+    or float4_e2m1fn_x2: two E2M1 elements a byte, the even one in the low
+    half) and scales [N, K/32] (uint8 or float8_e8m0fnu), both CUDA and
+    contiguous, K a multiple of 32.  With one argument, a bf16 / fp16 / fp32
+    weight [N, K], which is quantised first (mxfp4_quant)."""
+    _need(codes, "codes")
+    if scales is None:
+        if codes.dim() != 2 or codes.dtype not in _X_TYPES:
+            raise ValueError("a weight without scales must be [N, K] in bfloat16, float16 or float32")
+        _, scales, codes = mxfp4_quant(codes)
+    _need(scales, "scales")
+    if codes.dtype not in (torch.uint8, torch.int8, torch.float4_e2m1fn_x2) or codes.dim() != 2:
+        raise ValueError(f"codes must be [N, K/2] uint8, int8 or float4_e2m1fn_x2, got {codes.dtype} {tuple(codes.shape)}")
+    if scales.dtype not in (torch.uint8, torch.float8_e8m0fnu):
+        raise ValueError(f"scales must be uint8 or float8_e8m0fnu, got {scales.dtype}")
+    _contig(codes, "codes")
+    _contig(scales, "scales")
+    N, K = codes.shape[0], 2 * codes.shape[1]
+    if tuple(scales.shape) != (N, K // 32) or K % 32:
+        raise ValueError(f"scales {tuple(scales.shape)} do not match codes {tuple(codes.shape)}: [N, K/32] for K a "
+                         "multiple of 32")
+    _current(codes, scales)
+    nbytes = lib().dsa_linear_mxfp4_packed_bytes(N, K)
+    if nbytes == 0:
+        raise ValueError(f"weight [{N}, {K}]: sizes must be positive and at most 2^24")
+    packed = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
+    check(lib().dsa_linear_mxfp4_pack(codes.data_ptr(), scales.data_ptr(), N, K, packed.data_ptr(), nbytes,
+                                      _stream(codes)), "linear_mxfp4_pack")
+    return MXFP4Weight(packed, N, K)
+
+
+def linear_mxfp4(x: torch.Tensor, w: MXFP4Weight, out: torch.Tensor | None = None, out_f32: bool = False,
+                 ws: Workspace | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """``y[b, n] = q(x)[b] . W[n]`` on the 4-bit tensor cores
+    (dsa_linear_mxfp4): x [B, K] bf16, fp16 or fp32 (row stride a multiple of
+    16 bytes), quantised to MXFP4 in the call, ``w`` an MXFP4Weight -> y [B, N]
+    bf16, or the fp32 sums with ``out_f32``.  Without ``ws`` the scratch (x's
+    codes and scales) is allocated on the current stream for this call."""
+    _need(x, "x")
+    if x.dtype not in _X_TYPES:
+        raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
+    if not isinstance(w, MXFP4Weight):
+        raise TypeError("w must be an MXFP4Weight (pack_linear_weight_mxfp4)")
+    N, K = w.N, w.K
+    if x.dim() != 2 or x.shape[1] != K or x.stride(1) != 1:
+        raise ValueError(f"x must be [B, {K}] with contiguous rows, got {tuple(x.shape)}")
+    B = x.shape[0]
+    dtype = F32 if out_f32 else BF16
+    if out is None:
+        out = torch.empty(B, N, dtype=dtype, device=x.device)
+    else:
+        _need(out, "out", dtype)
+        if out.dim() != 2 or out.shape[0] != B or out.shape[1] < N or out.stride(1) != 1:
+            raise ValueError(f"out must be [{B}, >={N}] with contiguous rows, got {tuple(out.shape)}")
+    _current(x, w.packed, out, status)
+    if B == 0:
+        return out
+    L = lib()
+    need = L.dsa_linear_mxfp4_workspace_size(B, N, K)
+    buf = ws.get(need) if ws is not None else torch.empty(need, dtype=torch.uint8, device=x.device)
+    check(L.dsa_linear_mxfp4(x.data_ptr(), _X_TYPES[x.dtype], x.stride(0), w.packed.data_ptr(), out.data_ptr(),
+                             out.stride(0), B, N, K, int(out_f32), buf.data_ptr(), buf.numel(), _ptr(status),
+                             _stream(x)), "linear_mxfp4")
+    return out
+
+
 # ------------------------------------------------------------------ attn.kv
 
 def act_quant_block(x: torch.Tensor, block: int = 64, fp8_max: float = 448.0, eps: float = 1e-4,
