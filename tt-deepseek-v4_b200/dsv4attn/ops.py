@@ -20,8 +20,14 @@ I32 = torch.int32
 F32 = torch.float32
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _stream(t: torch.Tensor):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """cudaStream_t of the current stream on t's device (the handle of
+    torch.cuda.current_stream without building the Stream object: 0.1
+    against 2 us a call)."""
+    return _raw_stream(t.get_device())
 
 
 def _need(t: torch.Tensor, name: str, dtype=None, cuda=True):
@@ -223,13 +229,13 @@ def pack_linear_weight_mxfp4(codes: torch.Tensor, scales: torch.Tensor | None = 
     if tuple(scales.shape) != (N, K // 32) or K % 32:
         raise ValueError(f"scales {tuple(scales.shape)} do not match codes {tuple(codes.shape)}: [N, K/32] for K a "
                          "multiple of 32")
-    _current(codes, scales)
+    stream = _launch_stream(codes, scales)
     nbytes = lib().dsa_linear_mxfp4_packed_bytes(N, K)
     if nbytes == 0:
         raise ValueError(f"weight [{N}, {K}]: sizes must be positive and at most 2^24")
     packed = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
-    check(lib().dsa_linear_mxfp4_pack(codes.data_ptr(), scales.data_ptr(), N, K, packed.data_ptr(), nbytes,
-                                      _stream(codes)), "linear_mxfp4_pack")
+    check(lib().dsa_linear_mxfp4_pack(codes.data_ptr(), scales.data_ptr(), N, K, packed.data_ptr(), nbytes, stream),
+          "linear_mxfp4_pack")
     return MXFP4Weight(packed, N, K)
 
 
@@ -241,7 +247,8 @@ def linear_mxfp4(x: torch.Tensor, w: MXFP4Weight, out: torch.Tensor | None = Non
     bf16, or the fp32 sums with ``out_f32``.  Without ``ws`` the scratch (x's
     codes and scales) is allocated on the current stream for this call."""
     _need(x, "x")
-    if x.dtype not in _X_TYPES:
+    x_type = _X_TYPES.get(x.dtype)
+    if x_type is None:
         raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
     if not isinstance(w, MXFP4Weight):
         raise TypeError("w must be an MXFP4Weight (pack_linear_weight_mxfp4)")
@@ -251,20 +258,19 @@ def linear_mxfp4(x: torch.Tensor, w: MXFP4Weight, out: torch.Tensor | None = Non
     B = x.shape[0]
     dtype = F32 if out_f32 else BF16
     if out is None:
-        out = torch.empty(B, N, dtype=dtype, device=x.device)
+        out = x.new_empty((B, N), dtype=dtype)
     else:
         _need(out, "out", dtype)
         if out.dim() != 2 or out.shape[0] != B or out.shape[1] < N or out.stride(1) != 1:
             raise ValueError(f"out must be [{B}, >={N}] with contiguous rows, got {tuple(out.shape)}")
-    _current(x, w.packed, out, status)
+    stream = _launch_stream(x, w.packed, out, status)
     if B == 0:
         return out
     L = lib()
     need = L.dsa_linear_mxfp4_workspace_size(B, N, K)
-    buf = ws.get(need) if ws is not None else torch.empty(need, dtype=torch.uint8, device=x.device)
-    check(L.dsa_linear_mxfp4(x.data_ptr(), _X_TYPES[x.dtype], x.stride(0), w.packed.data_ptr(), out.data_ptr(),
-                             out.stride(0), B, N, K, int(out_f32), buf.data_ptr(), buf.numel(), _ptr(status),
-                             _stream(x)), "linear_mxfp4")
+    buf = ws.get(need) if ws is not None else x.new_empty(need, dtype=torch.uint8)
+    check(L.dsa_linear_mxfp4(x.data_ptr(), x_type, x.stride(0), w.packed.data_ptr(), out.data_ptr(), out.stride(0),
+                             B, N, K, out_f32, buf.data_ptr(), need, _ptr(status), stream), "linear_mxfp4")
     return out
 
 
@@ -300,27 +306,38 @@ def act_quant_block(x: torch.Tensor, block: int = 64, fp8_max: float = 448.0, ep
 _X_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def _rows2d(t: torch.Tensor, name: str) -> torch.Tensor:
-    """[..., K] as a view [M, K] with unit stride in the last dim."""
+def _row_stride(t: torch.Tensor, name: str) -> int:
+    """Row stride of t [..., K] read as a matrix of rows with unit stride in
+    the last dim."""
+    if t.is_contiguous():
+        return t.shape[-1]
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name} must have a unit stride in the last dim")
     try:
         t2 = t.view(-1, t.shape[-1])
     except RuntimeError:
         raise ValueError(f"{name} {tuple(t.shape)} with strides {t.stride()} is not a matrix of rows") from None
-    return t2
-
-
-def _ld(t2: torch.Tensor) -> int:
-    """Row stride of an [M, K] view; a single row's is never used."""
     return t2.stride(0) if t2.shape[0] > 1 else t2.shape[1]
 
 
-def _current(t: torch.Tensor, *others) -> None:
-    """The launch goes to the current device: the tensors must be on it."""
-    for o in (t, *others):
-        if o is not None and o.device.index != torch.cuda.current_device():
-            raise ValueError(f"tensor on {o.device}, current device is cuda:{torch.cuda.current_device()}")
+def _launch_stream(t: torch.Tensor, *others) -> int:
+    """The current stream of t's device.  Launches go to the current device:
+    t and the other tensors must be on it."""
+    dev = t.get_device()
+    cur = torch.cuda.current_device()
+    for o in others:
+        if o is not None and o.get_device() != dev:
+            raise ValueError(f"tensors on {t.device} and {o.device}")
+    if dev != cur:
+        raise ValueError(f"tensor on {t.device}, current device is cuda:{cur}")
+    return _raw_stream(dev)
+
+
+def _mx_field(t: torch.Tensor, name: str, shape: tuple) -> None:
+    _need(t, name, torch.uint8)
+    _contig(t, name)
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
 
 
 def mxfp4_quant(x: torch.Tensor, out=None, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None):
@@ -331,44 +348,49 @@ def mxfp4_quant(x: torch.Tensor, out=None, codes: torch.Tensor | None = None, sc
     half), scales [..., K/32] uint8, and the round-trip values in x's type
     when ``out`` is True or a tensor (which may be x), else None."""
     _need(x, "x")
-    if x.dtype not in _X_TYPES:
-        raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
-    K = x.shape[-1] if x.dim() else 0
+    dtype = x.dtype
+    x_type = _X_TYPES.get(dtype)
+    if x_type is None:
+        raise ValueError(f"x must be bfloat16, float16 or float32, got {dtype}")
+    *lead, K = x.shape if x.dim() else (0,)
     if K == 0 or K % 32:
         raise ValueError(f"last dim {K} must be a positive multiple of 32")
-    x2 = _rows2d(x, "x")
-    M = x2.shape[0]
+    ld, ld_out = _row_stride(x, "x"), 0
     if out is True:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    o2 = None
-    if out is not None:
-        _need(out, "out", x.dtype)
+        out, ld_out = x.new_empty(x.shape), K
+    elif out is not None:
+        _need(out, "out", dtype)
         if out.shape != x.shape:
             raise ValueError("out must have x's shape")
-        o2 = _rows2d(out, "out")
+        ld_out = _row_stride(out, "out")
     if codes is None:
-        codes = torch.empty(*x.shape[:-1], K // 2, dtype=torch.uint8, device=x.device)
+        codes = x.new_empty((*lead, K // 2), dtype=torch.uint8)
+    else:
+        _mx_field(codes, "codes", (*lead, K // 2))
     if scales is None:
-        scales = torch.empty(*x.shape[:-1], K // 32, dtype=torch.uint8, device=x.device)
-    for t, n, w in ((codes, "codes", K // 2), (scales, "scales", K // 32)):
-        _need(t, n, torch.uint8)
-        _contig(t, n)
-        if t.shape != (*x.shape[:-1], w):
-            raise ValueError(f"{n} must be {(*x.shape[:-1], w)}, got {tuple(t.shape)}")
-    _current(x, out, codes, scales)
-    if M == 0:
-        return out, scales, codes
-    check(lib().dsa_mxfp4_quant(x2.data_ptr(), _X_TYPES[x.dtype], _ld(x2), _ptr(o2), _ld(o2) if o2 is not None else 0,
-                                codes.data_ptr(), scales.data_ptr(), M, K, _stream(x)), "mxfp4_quant")
+        scales = x.new_empty((*lead, K // 32), dtype=torch.uint8)
+    else:
+        _mx_field(scales, "scales", (*lead, K // 32))
+    stream = _launch_stream(x, out, codes, scales)
+    M = x.numel() // K
+    if M:
+        check(lib().dsa_mxfp4_quant(x.data_ptr(), x_type, ld, _ptr(out), ld_out, codes.data_ptr(), scales.data_ptr(),
+                                    M, K, stream), "mxfp4_quant")
     return out, scales, codes
+
+
+_row_bytes: dict = {}  # (D, rope_dim) -> bytes, the sizes in use
 
 
 def kv_quant_row_bytes(D: int = 512, rope_dim: int = 64) -> int:
     """Bytes of one record of the FP8 latent cache (608 for 448 + 64 dims)."""
-    n = int(lib().dsa_kv_quant_row_bytes(D, rope_dim))
-    if n == 0:
-        raise ValueError(f"D={D}, rope_dim={rope_dim}: D - rope_dim must be a positive multiple of 64, rope_dim a "
-                         "multiple of 8, D <= 8192")
+    n = _row_bytes.get((D, rope_dim))
+    if n is None:
+        n = int(lib().dsa_kv_quant_row_bytes(D, rope_dim))
+        if n == 0:
+            raise ValueError(f"D={D}, rope_dim={rope_dim}: D - rope_dim must be a positive multiple of 64, rope_dim a "
+                             "multiple of 8, D <= 8192")
+        _row_bytes[D, rope_dim] = n
     return n
 
 
@@ -385,15 +407,16 @@ def kv_quant_views(cache: torch.Tensor, D: int = 512, rope_dim: int = 64):
         raise ValueError(f"cache must be uint8 with records of {kv_quant_row_bytes(D, rope_dim)} bytes")
     a = D - rope_dim
     b = a + 2 * rope_dim
-    return (cache[..., :a].view(torch.float8_e4m3fn), cache[..., a:b].view(BF16),
-            cache[..., b:b + a // 16].view(F32))
+    return (cache.narrow(-1, 0, a).view(torch.float8_e4m3fn), cache.narrow(-1, a, b - a).view(BF16),
+            cache.narrow(-1, b, a // 16).view(F32))
 
 
 def _quant_cache(cache: torch.Tensor, B: int, D: int, rope_dim: int) -> None:
     _need(cache, "cache", torch.uint8)
     rb = kv_quant_row_bytes(D, rope_dim)
-    if cache.dim() != 3 or cache.shape[0] < B or cache.shape[2] != rb or cache.shape[1] < 1 \
-            or cache.stride(2) != 1 or (cache.shape[1] > 1 and cache.stride(1) != rb):
+    shape = cache.shape
+    if len(shape) != 3 or shape[0] < B or shape[2] != rb or shape[1] < 1 \
+            or cache.stride()[1:] != (rb, 1) and (cache.stride(2) != 1 or shape[1] > 1):
         raise ValueError(f"cache must be [>={B}, rows, {rb}] with contiguous rows (D={D}, rope_dim={rope_dim}), "
                          f"got {tuple(cache.shape)}")
 
@@ -419,16 +442,16 @@ def kv_quant_write(kv: torch.Tensor, cache: torch.Tensor, pos: torch.Tensor, win
     if kv.dim() != 3 or kv.stride(2) != 1:
         raise ValueError("kv must be [B, S, D] or [B, D] with a unit stride in the last dim")
     B, S, D = kv.shape
+    ld_b, ld_s, _ = kv.stride()
     _quant_cache(cache, B, D, rope_dim)
     _per_sequence(pos, "pos", B)
     if n_valid is not None:
         _per_sequence(n_valid, "n_valid", B)
-    _current(kv, cache, pos, n_valid)
-    if kv.numel() == 0:
-        return
-    check(lib().dsa_kv_quant_write(kv.data_ptr(), kv.stride(0), kv.stride(1), cache.data_ptr(), cache.stride(0),
-                                   cache.shape[1], pos.data_ptr(), _ptr(n_valid), B, S, D, rope_dim, win, offset,
-                                   _stream(kv)), "kv_quant_write")
+    stream = _launch_stream(kv, cache, pos, n_valid)
+    if B and S:
+        check(lib().dsa_kv_quant_write(kv.data_ptr(), ld_b, ld_s, cache.data_ptr(), cache.stride(0), cache.shape[1],
+                                       pos.data_ptr(), _ptr(n_valid), B, S, D, rope_dim, win, offset, stream),
+              "kv_quant_write")
 
 
 def kv_quant_read(cache: torch.Tensor, idx: torch.Tensor | None = None, D: int = 512, rope_dim: int = 64,
@@ -449,16 +472,16 @@ def kv_quant_read(cache: torch.Tensor, idx: torch.Tensor | None = None, D: int =
         K = idx.shape[1]
         ld = idx.stride(0) if B > 1 else K
     if out is None:
-        out = torch.empty(B, K, D, dtype=dtype, device=cache.device)
-    _need(out, "out", dtype)
-    _contig(out, "out")
-    if tuple(out.shape) != (B, K, D):
-        raise ValueError(f"out must be {(B, K, D)}, got {tuple(out.shape)}")
-    _current(cache, idx, out, status)
-    if out.numel() == 0:
-        return out
-    check(lib().dsa_kv_quant_read(cache.data_ptr(), cache.stride(0), cache.shape[1], _ptr(idx), ld, out.data_ptr(),
-                                  int(dtype == F32), B, K, D, rope_dim, _ptr(status), _stream(cache)), "kv_quant_read")
+        out = cache.new_empty((B, K, D), dtype=dtype)
+    else:
+        _need(out, "out", dtype)
+        _contig(out, "out")
+        if out.shape != (B, K, D):
+            raise ValueError(f"out must be {(B, K, D)}, got {tuple(out.shape)}")
+    stream = _launch_stream(cache, idx, out, status)
+    if B and K:
+        check(lib().dsa_kv_quant_read(cache.data_ptr(), cache.stride(0), cache.shape[1], _ptr(idx), ld, out.data_ptr(),
+                                      dtype == F32, B, K, D, rope_dim, _ptr(status), stream), "kv_quant_read")
     return out
 
 
@@ -985,39 +1008,41 @@ def sparse_attn_quant(q, cache, idx, sink, scale: float, out=None, lse=None, ws:
     _need(idx, "idx", I32)
     _need(sink, "sink", F32)
     _contig(sink, "sink")
-    if q.dim() not in (3, 4):
+    *lead, H, D = q.shape if q.dim() >= 2 else (0, 0)
+    if len(lead) not in (1, 2):
         raise ValueError("q must be [B, S, H, D] or [B, H, D]")
-    B, S, (H, D) = q.shape[0], q.shape[1] if q.dim() == 4 else 1, q.shape[-2:]
-    if (H, D) != (64, 512) or sink.numel() != H:
+    if H != 64 or D != 512 or sink.numel() != H:
         raise ValueError(f"sparse_attn_quant: built for 64 heads of 512 dims and as many sinks (got {H} of {D}, "
                          f"{sink.numel()} sinks)")
+    B, S = lead[0], lead[1] if len(lead) == 2 else 1
     _quant_cache(cache, B, D, 64)
-    K = idx.shape[-1]
-    if tuple(idx.shape[:-1]) not in ((B, S), (B,) if S == 1 else (B, S)):
+    *ilead, K = idx.shape if idx.dim() else (0,)
+    if ilead != lead and (S != 1 or ilead not in ([B], [B, 1])):
         raise ValueError(f"idx must be [B, S, K] for q {tuple(q.shape)}, got {tuple(idx.shape)}")
-    idx2 = _rows2d(idx, "idx") if idx.numel() else idx.reshape(B * S, K)
+    ld_idx = _row_stride(idx, "idx") if K else 0
     if out is None:
         out = torch.empty_like(q)
-    _need(out, "out", BF16)
-    _contig(out, "out")
-    if out.shape != q.shape:
-        raise ValueError("out must have q's shape")
+    else:
+        _need(out, "out", BF16)
+        _contig(out, "out")
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
     if lse is not None:
         _need(lse, "lse", F32)
         _contig(lse, "lse")
         if lse.numel() != B * S * H:
             raise ValueError(f"lse has {lse.numel()} elements, expected {B * S * H}")
-    _current(q, cache, idx, sink, out, lse, status)
-    if q.numel() == 0:
+    stream = _launch_stream(q, cache, idx, sink, out, lse, status)
+    if B == 0 or S == 0:
         return out
     L = lib()
     need = L.dsa_sparse_attn_workspace_size(B, S, H, D, K)
     buf = None
     if need:
-        buf = ws.get(need) if ws is not None else torch.empty(need, dtype=torch.uint8, device=q.device)
+        buf = ws.get(need) if ws is not None else q.new_empty(need, dtype=torch.uint8)
     check(L.dsa_sparse_attn_quant(q.data_ptr(), cache.data_ptr(), cache.stride(0), cache.shape[1],
-                                  idx2.data_ptr() if K else sink.data_ptr(), _ld(idx2), sink.data_ptr(), out.data_ptr(), _ptr(lse), B, S, H, D, K, scale,
-                                  _ptr(buf), need if buf is not None else 0, _ptr(status), _stream(q)),
+                                  idx.data_ptr() if K else sink.data_ptr(), ld_idx, sink.data_ptr(), out.data_ptr(),
+                                  _ptr(lse), B, S, H, D, K, scale, _ptr(buf), need, _ptr(status), stream),
           "sparse_attn_quant")
     return out
 
