@@ -19,18 +19,31 @@ __host__ __device__ constexpr int row_bytes(int nope, int rope) {
   return (nope + 2 * rope + 4 * (nope / kBlock) + 31) / 32 * 32;
 }
 
-// 8 e4m3 codes times their scale, rounded to bf16 once.  e4m3 -> fp16 is
-// exact, fp16 -> fp32 too, and the fp32 product is the one kv_window_write
-// rounds.  (A code is never NaN: kv_quant_write marks a block that holds a
-// NaN or an infinity by a NaN scale.)
+// 8 e4m3 codes times their scale in fp32: e4m3 -> fp16 -> fp32 is exact, so
+// the product is the one kv_window_write rounds.  (A code is never NaN:
+// kv_quant_write marks a block that holds a NaN or an infinity by a NaN
+// scale.)  Two products an instruction (mul.f32x2).
 __device__ __forceinline__ void values8(uint2 codes, float s, float* v) {
   const uint32_t w[2] = {codes.x, codes.y};
+  uint64_t s2;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(s));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t((w[i >> 1] >> (16 * (i & 1))) & 0xffffu), __NV_E4M3);
-    const float2 f = __half22float2(__half2(h));
-    v[2 * i] = f.x * s;
-    v[2 * i + 1] = f.y * s;
+  for (int i = 0; i < 2; ++i) {
+    uint32_t h[2];
+    asm("{\n\t.reg .b16 lo, hi;\n\t"
+        "mov.b32 {lo, hi}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, lo;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(h[0]), "=r"(h[1])
+        : "r"(w[i]));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+      uint64_t x;
+      asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(f.x), "f"(f.y));
+      asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(x) : "l"(x), "l"(s2));
+      asm("mov.b64 {%0, %1}, %2;" : "=f"(v[4 * i + 2 * j]), "=f"(v[4 * i + 2 * j + 1]) : "l"(x));
+    }
   }
 }
 

@@ -291,6 +291,7 @@ static int sparse_attn_run(const void* q, const void* kv, int64_t kv_bstride, in
   }
   DSA_CHECK_ARG(quant || kv_bstride % kSaD == 0, "sparse_attn: kv batch stride must be a multiple of D");
   const int64_t row_stride = quant ? kv_bstride : kv_bstride / kSaD;
+  const int threads = quant ? satc::kQuantThreads : satc::THREADS;
   auto kernel = quant ? satc::sparse_attn_tc_kernel<true> : satc::sparse_attn_tc_kernel<false>;
   CUtensorMap tm_q;
   if (!tma::make_2d_bf16(&tm_q, q, kSaD, uint64_t(M) * kSaH, kSaD * 2, 64, 64)) {
@@ -300,7 +301,7 @@ static int sparse_attn_run(const void* q, const void* kv, int64_t kv_bstride, in
   if (pair) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2, M);
-    cfg.blockDim = dim3(satc::THREADS);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = satc::kSmemBytes;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -316,7 +317,7 @@ static int sparse_attn_run(const void* q, const void* kv, int64_t kv_bstride, in
     DSA_CHECK_LAUNCH("sparse_attn");
     return DSA_OK;
   }
-  launch_pdl(kernel, dim3(p.nsplit, M), dim3(satc::THREADS), satc::kSmemBytes, st, t, tm_q, row_stride);
+  launch_pdl(kernel, dim3(p.nsplit, M), dim3(threads), satc::kSmemBytes, st, t, tm_q, row_stride);
   DSA_CHECK_LAUNCH("sparse_attn");
   if (p.nsplit > 1) {
     launch_lse_combine(ws_ml, ws_o, true, sink, p.nsplit, M, kSaH, kSaD, final_mode ? 1 : 0,

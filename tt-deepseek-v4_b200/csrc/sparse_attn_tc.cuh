@@ -57,12 +57,11 @@
 //               tcgen05.st), after which the slot takes its first tile.
 //
 // kQuant: the rows are records of the FP8 latent cache (kv_quant_dev.cuh).
-// The producers load a record's codes, scales and rotary dims into registers,
-// expand them to the bf16 rows of the tile and store those where the copies
-// of the bf16 cache land; everything behind the tile is the same.  Registers,
-// not a staging ring: the three 64 KB slots leave 3 KB of shared memory.  A
-// warp keeps two groups of four rows, the next group's loads in flight while
-// it expands the one before.
+// Thirteen producer warps load a record's codes, scales and rotary dims into
+// registers, expand them to the bf16 rows of the tile and store those where
+// the copies of the bf16 cache land; everything behind the tile is the same.
+// Registers, not a staging ring: the three 64 KB slots leave 5 KB of shared
+// memory.  As a warp stores a row of tile t it requests its row of t + 1.
 //
 // Every mbarrier wait is bounded (about a second); a wait that runs out sets
 // a status bit and an abort flag that makes all later waits of the CTA return
@@ -95,15 +94,18 @@ constexpr int kPairBytes = 2 * kSlabBytes;            // 16 KB
 constexpr int kProducerWarps = 9;
 constexpr int kMmaWarp = 4;
 constexpr int THREADS = 512;
-__device__ __forceinline__ bool is_producer_warp(int w) { return w >= 5 && (w & 3) != 0; }
-__device__ __forceinline__ int producer_index(int w) { return w - 5 - ((w - 4) >> 2); }
+// kQuant: expanding a tile takes instructions, so four more producer warps
+// (16-19), one on each scheduler
+constexpr int kQuantThreads = 640;
+constexpr int kQuantProducerWarps = 13;
+__device__ __forceinline__ bool is_producer_warp(int w) { return w >= 16 || (w >= 5 && (w & 3) != 0); }
+__device__ __forceinline__ int producer_index(int w) { return w >= 16 ? w - 7 : w - 5 - ((w - 4) >> 2); }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescaleThreshold = 8.0f;             // log2 units
 constexpr int kPBytes = H * TK * 2;                   // 8 KB per buffer: [64 heads x 64 keys] bf16
 constexpr int kMaxTilesPerSplit = 36;
 constexpr int kIdxCap = kMaxTilesPerSplit * TK;       // indices staged per split
-constexpr int kIdxPerThread = (kIdxCap + THREADS - 1) / THREADS;
 constexpr int kAuxBytes = 4096;
 constexpr int kOffRing = 0;
 constexpr int kOffP = kOffRing + NT * kTileBytes;
@@ -121,16 +123,16 @@ constexpr int kPairXFloats = 8 * D * 4 + 64;
 constexpr int kRope = 64;
 constexpr int kNope = D - kRope;
 constexpr int kRecBytes = kvq::row_bytes(kNope, kRope);
-constexpr int kGroup = 4;                             // rows a producer warp loads at a time (kQuant)
-constexpr int kGroups = 2;                            // groups a tile: kGroup * kGroups * kProducerWarps >= TK
+constexpr int kQuantRows = 5;                         // rows of a tile a producer warp expands (kQuant)
 constexpr uint32_t kIdescS = tc::idesc_bf16(128, 128, false, false);
 constexpr uint32_t kIdescPV = tc::idesc_bf16(128, 64, true, false);
 static_assert(kSmemBytes <= 232448, "shared memory budget");
 static_assert(kColS + 128 <= kTmemCols, "TMEM columns");
-static_assert(kGroup * kGroups * kProducerWarps >= TK, "a producer warp's rows of a tile");
+static_assert(kQuantRows * kQuantProducerWarps >= TK, "a producer warp's rows of a tile");
 static_assert(kNope / 8 == 56 && kRope / 8 == 8, "a lane's two chunks of a record: 56 of codes, 8 of rotary dims");
 static_assert(TK == 64, "the block-diagonal layout assumes 64-key tiles");
 static_assert(kIdxCap % 32 == 0 && THREADS % 32 == 0, "index staging ballots whole warps");
+static_assert(kQuantThreads == 32 * (16 + 4) && kQuantProducerWarps == kProducerWarps + 4, "warps 16-19 are producers");
 
 enum : int { kStatusBadIndex = 1, kStatusTimeout = 2 };
 
@@ -256,38 +258,33 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// One group of a producer warp's rows of a tile, as the lane's two chunks of
-// 8 dims each: chunk lane (codes) and chunk lane + 32 (codes below lane 24,
-// rotary dims from there)
-struct RecGroup {
-  uint2 lo[kGroup];
-  uint4 hi[kGroup];
-  float s_lo[kGroup], s_hi[kGroup];
+// A record as the lane's two chunks of 8 dims: chunk lane (codes) and chunk
+// lane + 32 (codes below lane 24, rotary dims from there: all of hi)
+struct RecPart {
+  uint2 lo;
+  uint4 hi;
+  float s_lo, s_hi;
 };
 
-// rows pw, pw + P, ... (the group's kGroup of them) of the tile whose indices
-// start at idx; a masked row and a row past the tile are all zero
-__device__ __forceinline__ void load_group(RecGroup& r, const uint8_t* kvb, const int32_t* idx, int row0, int lane) {
-#pragma unroll
-  for (int i = 0; i < kGroup; ++i) {
-    const int row = row0 + i * kProducerWarps;
-    const int id = row < TK ? idx[row] : -1;
-    r.lo[i] = make_uint2(0, 0);
-    r.hi[i] = make_uint4(0, 0, 0, 0);
-    r.s_lo[i] = r.s_hi[i] = 0.f;
-    if (id >= 0) {
-      const uint8_t* rec = kvb + int64_t(id) * kRecBytes;
-      const float* scales = reinterpret_cast<const float*>(rec + kNope + 2 * kRope);
-      r.lo[i] = __ldg(reinterpret_cast<const uint2*>(rec) + lane);
-      r.s_lo[i] = __ldg(scales + (lane >> 3));
-      if (lane < 24) {
-        const uint2 w = __ldg(reinterpret_cast<const uint2*>(rec) + 32 + lane);
-        r.hi[i].x = w.x;
-        r.hi[i].y = w.y;
-        r.s_hi[i] = __ldg(scales + 4 + (lane >> 3));
-      } else {
-        r.hi[i] = __ldg(reinterpret_cast<const uint4*>(rec + kNope) + (lane - 24));
-      }
+// record `id`, all zero where id < 0 (a masked row).  hi_off: the lane's
+// second chunk in a record.
+__device__ __forceinline__ void load_record(RecPart& r, const uint8_t* recs, int id, int lane, uint32_t hi_off) {
+  r.lo = make_uint2(0, 0);
+  r.hi = make_uint4(0, 0, 0, 0);
+  r.s_lo = r.s_hi = 0.f;
+  if (id >= 0) {
+    const uint8_t* rec = recs + int64_t(id) * kRecBytes;
+    const float* scales = reinterpret_cast<const float*>(rec + kNope + 2 * kRope) + (lane >> 3);
+    r.lo = __ldg(reinterpret_cast<const uint2*>(rec) + lane);
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(rec + hi_off));
+    r.hi.x = w.x;
+    r.hi.y = w.y;
+    r.s_lo = __ldg(scales);
+    r.s_hi = __ldg(scales + 4);  // (lanes 24..31: the record's padding)
+    if (lane >= 24) {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(rec + hi_off + 8));
+      r.hi.z = u.x;
+      r.hi.w = u.y;
     }
   }
 }
@@ -297,22 +294,23 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, const uint4& v) {
                : "memory");
 }
 
-__device__ __forceinline__ void store_group(const RecGroup& r, uint32_t tile, int row0, int lane) {
-#pragma unroll
-  for (int i = 0; i < kGroup; ++i) {
-    const int row = row0 + i * kProducerWarps;
-    if (row < TK) {
-      st_shared16(tile + chunk_off(row, lane), kvq::bf16_values8(r.lo[i], r.s_lo[i]));
-      const uint4 h = lane < 24 ? kvq::bf16_values8(make_uint2(r.hi[i].x, r.hi[i].y), r.s_hi[i]) : r.hi[i];
-      st_shared16(tile + chunk_off(row, lane + 32), h);
-    }
-  }
+// Key k of the tile.  tile_lane: chunk_off(0, lane) without its swizzle, from
+// the tile's start.  Both chunks of a lane have the same swizzle, the second
+// lies 16 rows on.
+__device__ __forceinline__ void store_record(const RecPart& r, uint32_t tile_lane, int k, int lane) {
+  const uint32_t at = tile_lane + (k + (k & ~15)) * 128 + (((lane ^ k) & 7) << 4);
+  st_shared16(at, kvq::bf16_values8(r.lo, r.s_lo));
+  // (rotary lanes: converted for nothing, without a branch)
+  uint4 h = kvq::bf16_values8(make_uint2(r.hi.x, r.hi.y), r.s_hi);
+  if (lane >= 24) h = r.hi;
+  st_shared16(at + 16 * 128, h);
 }
 
 template <bool kQuant>
-__global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a,
-                                                                    const __grid_constant__ CUtensorMap tm_q,
-                                                                    int64_t kv_row_base_stride) {
+__global__ void __launch_bounds__(kQuant ? kQuantThreads : THREADS, 1)
+    sparse_attn_tc_kernel(const Args a, const __grid_constant__ CUtensorMap tm_q, int64_t kv_row_base_stride) {
+  constexpr int kThreads = kQuant ? kQuantThreads : THREADS;
+  constexpr int kIdxPerThread = (kIdxCap + kThreads - 1) / kThreads;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Aux* aux = reinterpret_cast<Aux*>(smem + kOffAux);
@@ -344,10 +342,10 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a
   }
   if (tid == 32) {
     tc::mbar_init(smem_u32(&aux->q_tma), 1);
-    tc::mbar_init(smem_u32(&aux->q_full), THREADS);  // every thread stores its part of Q'
+    tc::mbar_init(smem_u32(&aux->q_full), THREADS);  // every thread of warps 0-15 stores its part of Q'
     for (int s = 0; s < NT; ++s) {
       // one cp.async arrival per producer lane; kQuant: one of each producer warp
-      tc::mbar_init(smem_u32(&aux->full[s]), kQuant ? kProducerWarps : 32 * kProducerWarps);
+      tc::mbar_init(smem_u32(&aux->full[s]), kQuant ? kQuantProducerWarps : 32 * kProducerWarps);
       tc::mbar_init(smem_u32(&aux->empty[s]), 2);  // both PV issuers' commits
     }
     tc::mbar_init(smem_u32(&aux->s_full), 1);
@@ -422,6 +420,7 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a
   };
   // every warp moves its part of Q' once the TMA copy has landed
   auto q_part = [&]() {
+    if (kQuant && warp >= 16) return;
     warp_wait(&aux->q_tma, 0);
     q_part_to_tmem(sQstage, tmem, warp, lane, &aux->q_full);
   };
@@ -448,12 +447,12 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a
     int ids[kIdxPerThread];
 #pragma unroll
     for (int k = 0; k < kIdxPerThread; ++k) {
-      const int e = tid + k * THREADS;
+      const int e = tid + k * kThreads;
       ids[k] = (e >= e0 && e < n * TK) ? index_at(e) : -1;
     }
 #pragma unroll
     for (int k = 0; k < kIdxPerThread; ++k) {
-      const int e = tid + k * THREADS;
+      const int e = tid + k * kThreads;
       if (e >= e0 && e < n * TK) {  // whole warps: n * TK and e0 are multiples of 64
         stage(e, ids[k]);
       }
@@ -472,22 +471,28 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a
     const int pw = producer_index(warp);
     if constexpr (kQuant) {
       const uint8_t* recs = static_cast<const uint8_t*>(a.kv) + int64_t(b) * kv_row_base_stride;
-      RecGroup g[kGroups];
+      const uint32_t hi_off = lane < 24 ? 256 + 8 * lane : kNope + 16 * (lane - 24);
+      const uint32_t lane_off = (lane >> 3) * kPairBytes;
+      RecPart rec[kQuantRows];
 #pragma unroll
-      for (int j = 0; j < kGroups; ++j)
-        if (n > 0) load_group(g[j], recs, s_idx, pw + j * kGroup * kProducerWarps, lane);
+      for (int i = 0; i < kQuantRows; ++i) {
+        const int k = pw + i * kQuantProducerWarps;
+        if (n > 0 && k < TK) load_record(rec[i], recs, s_idx[k], lane, hi_off);
+      }
       for (int t = 0; t < n; ++t) {
         if (t == NT - 1) {
           if (q_late) q_part();
           warp_wait(&aux->q_full, 0);
         }
         if (t >= NT) warp_wait(&aux->empty[t % NT], ((t / NT) - 1) & 1);
-        const uint32_t dst = sRing + (t % NT) * kTileBytes;
+        const uint32_t dst = sRing + (t % NT) * kTileBytes + lane_off;
 #pragma unroll
-        for (int j = 0; j < kGroups; ++j) {
-          const int row0 = pw + j * kGroup * kProducerWarps;
-          store_group(g[j], dst, row0, lane);
-          if (t + 1 < n) load_group(g[j], recs, s_idx + (t + 1) * TK, row0, lane);
+        for (int i = 0; i < kQuantRows; ++i) {
+          const int k = pw + i * kQuantProducerWarps;
+          if (k < TK) {
+            store_record(rec[i], dst, k, lane);
+            if (t + 1 < n) load_record(rec[i], recs, s_idx[(t + 1) * TK + k], lane, hi_off);
+          }
         }
         tc::fence_proxy_async();  // the tile is read by the tensor cores
         __syncwarp();
@@ -745,6 +750,7 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a
   __syncthreads();
   tc::fence_after_sync();
   if (tid == 0) SA_TRACE(kTrMisc, 3);
+  const bool drains = !kQuant || warp < 16;
   if (a.pair_combine) {
     // ------------------------------------------------------ pair combine
     // The row's splits 0 and 1 are this cluster's two CTAs (cluster rank =
@@ -769,7 +775,7 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a
     // [4 groups of 8 heads][D dims] x 16 B of bf16
     uint4* x_out = reinterpret_cast<uint4*>(a.pair_x + (int64_t(mrow) * 2 + pr) * kPairXFloats);
     const uint4* x_in = reinterpret_cast<const uint4*>(a.pair_x + (int64_t(mrow) * 2 + r) * kPairXFloats);
-    {
+    if (drains) {
       float o[32];
       if (n > 0) {
         tc::tmem_ld32(tl + kColO + H * jb + 32 * pr, o);
@@ -791,7 +797,7 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a
     // this CTA's own half and the sinks are read while the partner may
     // still be on its last tiles
     float own[32], peer[32];
-    if (n > 0) {
+    if (n > 0 && drains) {
       tc::tmem_ld32(tl + kColO + H * jb + 32 * r, own);
       tc::tmem_wait_ld();
     } else {
@@ -802,7 +808,7 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a
     cluster_sync();  // the last access of either CTA's shared memory by the other
     uint4 xp[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) xp[c] = __ldcg(x_in + c * D + d);
+    for (int c = 0; c < 4; ++c) xp[c] = drains ? __ldcg(x_in + c * D + d) : make_uint4(0, 0, 0, 0);
     if (tid < 32) {
       const int h = 32 * r + tid;
       const float mo = aux->m_fin[h], lo = aux->l_fin[h], mp = aux->peer_ml[2 * tid], lp = aux->peer_ml[2 * tid + 1];
@@ -826,23 +832,25 @@ __global__ void __launch_bounds__(THREADS, 1) sparse_attn_tc_kernel(const Args a
       }
     }
     __syncthreads();  // coefficients
-    // out[h][d]: lanes d, d ^ 1 trade one value per head pair so that each
-    // store writes two adjacent dims (even lane: head i, odd lane: head i + 1)
-    __nv_bfloat16* om = a.out + (int64_t(mrow) * H + 32 * r) * D;
-    const bool odd = lane & 1;
+    if (drains) {
+      // out[h][d]: lanes d, d ^ 1 trade one value per head pair so that each
+      // store writes two adjacent dims (even lane: head i, odd lane: head i + 1)
+      __nv_bfloat16* om = a.out + (int64_t(mrow) * H + 32 * r) * D;
+      const bool odd = lane & 1;
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const float x0a = r == 0 ? own[i] : peer[i], x1a = r == 0 ? peer[i] : own[i];
-      const float x0b = r == 0 ? own[i + 1] : peer[i + 1], x1b = r == 0 ? peer[i + 1] : own[i + 1];
-      const float va = fmaf(aux->coef[1][i], x1a, aux->coef[0][i] * x0a);
-      const float vb = fmaf(aux->coef[1][i + 1], x1b, aux->coef[0][i + 1] * x0b);
-      const float got = __shfl_xor_sync(0xffffffffu, odd ? va : vb, 1);
-      if (odd)
-        *reinterpret_cast<uint32_t*>(om + (i + 1) * D + d - 1) = pack_bf16x2(got, vb);
-      else
-        *reinterpret_cast<uint32_t*>(om + i * D + d) = pack_bf16x2(va, got);
+      for (int i = 0; i < 32; i += 2) {
+        const float x0a = r == 0 ? own[i] : peer[i], x1a = r == 0 ? peer[i] : own[i];
+        const float x0b = r == 0 ? own[i + 1] : peer[i + 1], x1b = r == 0 ? peer[i + 1] : own[i + 1];
+        const float va = fmaf(aux->coef[1][i], x1a, aux->coef[0][i] * x0a);
+        const float vb = fmaf(aux->coef[1][i + 1], x1b, aux->coef[0][i + 1] * x0b);
+        const float got = __shfl_xor_sync(0xffffffffu, odd ? va : vb, 1);
+        if (odd)
+          *reinterpret_cast<uint32_t*>(om + (i + 1) * D + d - 1) = pack_bf16x2(got, vb);
+        else
+          *reinterpret_cast<uint32_t*>(om + i * D + d) = pack_bf16x2(va, got);
+      }
     }
-  } else {
+  } else if (drains) {
     const int sp = warp & 3, jb = warp >> 2;
     const uint32_t tl = tmem + ((uint32_t)(32 * sp) << 16);
     const int d = 128 * jb + 32 * sp + lane;
