@@ -92,14 +92,25 @@ constexpr int kPairBytes = 2 * kSlabBytes;            // 16 KB
 // S issuer 8, and the producers on the schedulers of warps 1-3 only (5-7,
 // 9-11, 13-15), so the issuers share their scheduler with one softmax warp.
 constexpr int kProducerWarps = 9;
-constexpr int kMmaWarp = 4;
+__device__ __forceinline__ bool is_producer_warp(int w) { return w >= 5 && (w & 3) != 0; }
+__device__ __forceinline__ int producer_index(int w) { return w - 5 - ((w - 4) >> 2); }
 constexpr int THREADS = 512;
-// kQuant: expanding a tile takes instructions, so four more producer warps
-// (16-19), one on each scheduler
+// kQuant: expanding a tile takes instructions, so twenty warps, and every
+// scheduler gets its share of the 13 producers: softmax 0-3, issuers 4 (PV),
+// 9 (S) and 14 (PV) on three schedulers, producers the rest.  (The issuers on
+// one scheduler, as above, left four producers on each of the other three.)
 constexpr int kQuantThreads = 640;
 constexpr int kQuantProducerWarps = 13;
-__device__ __forceinline__ bool is_producer_warp(int w) { return w >= 16 || (w >= 5 && (w & 3) != 0); }
-__device__ __forceinline__ int producer_index(int w) { return w >= 16 ? w - 7 : w - 5 - ((w - 4) >> 2); }
+template <bool kQuant>
+struct Roles {
+  static constexpr int kPV0 = 4, kS = kQuant ? 9 : 8, kPV1 = kQuant ? 14 : 12;  // PV of dims 0-255, S, PV of 256-511
+  static __device__ __forceinline__ bool producer(int w) {
+    return kQuant ? w >= 5 && w != kS && w != kPV1 : is_producer_warp(w);
+  }
+  static __device__ __forceinline__ int index(int w) {
+    return kQuant ? w - 5 - int(w > kS) - int(w > kPV1) : producer_index(w);
+  }
+};
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescaleThreshold = 8.0f;             // log2 units
@@ -132,7 +143,7 @@ static_assert(kQuantRows * kQuantProducerWarps >= TK, "a producer warp's rows of
 static_assert(kNope / 8 == 56 && kRope / 8 == 8, "a lane's two chunks of a record: 56 of codes, 8 of rotary dims");
 static_assert(TK == 64, "the block-diagonal layout assumes 64-key tiles");
 static_assert(kIdxCap % 32 == 0 && THREADS % 32 == 0, "index staging ballots whole warps");
-static_assert(kQuantThreads == 32 * (16 + 4) && kQuantProducerWarps == kProducerWarps + 4, "warps 16-19 are producers");
+static_assert(kQuantThreads == 32 * (4 + 3 + kQuantProducerWarps), "softmax, issuers, producers");
 
 enum : int { kStatusBadIndex = 1, kStatusTimeout = 2 };
 
@@ -309,6 +320,7 @@ __device__ __forceinline__ void store_record(const RecPart& r, uint32_t tile_lan
 template <bool kQuant>
 __global__ void __launch_bounds__(kQuant ? kQuantThreads : THREADS, 1)
     sparse_attn_tc_kernel(const Args a, const __grid_constant__ CUtensorMap tm_q, int64_t kv_row_base_stride) {
+  using R = Roles<kQuant>;
   constexpr int kThreads = kQuant ? kQuantThreads : THREADS;
   constexpr int kIdxPerThread = (kIdxCap + kThreads - 1) / kThreads;
   extern __shared__ uint8_t smem_raw[];
@@ -429,7 +441,7 @@ __global__ void __launch_bounds__(kQuant ? kQuantThreads : THREADS, 1)
     load_q();
     if (tid < TK) stage(tid, index_at(tid));
     __syncthreads();
-    if (is_producer_warp(warp)) issue_tile(0, producer_index(warp));
+    if (R::producer(warp)) issue_tile(0, R::index(warp));
   } else if (a.early) {
     load_q();
   }
@@ -464,28 +476,40 @@ __global__ void __launch_bounds__(kQuant ? kQuantThreads : THREADS, 1)
   if (tid == 0) SA_TRACE(kTrMisc, 5);
   const bool q_late = !a.early;  // Q' still to be moved (q was loaded after the wait)
 
-  if (is_producer_warp(warp)) {
+  if (R::producer(warp)) {
     // ------------------------------------------------------------ producers
     // Tiles 0 .. NT-2 are requested first; the last slot holds the query
     // block until every thread has moved its part of Q' (q_full).
-    const int pw = producer_index(warp);
+    const int pw = R::index(warp);
     if constexpr (kQuant) {
       const uint8_t* recs = static_cast<const uint8_t*>(a.kv) + int64_t(b) * kv_row_base_stride;
       const uint32_t hi_off = lane < 24 ? 256 + 8 * lane : kNope + 16 * (lane - 24);
       const uint32_t lane_off = (lane >> 3) * kPairBytes;
+      // lane 6 i + j requests the j-th 128-byte line of the warp's i-th record
+      // of tile t into L2
+      auto prefetch_tile = [&](int t) {
+        const int i = lane / 6, k = pw + i * kQuantProducerWarps;
+        if (t < n && i < kQuantRows && k < TK) {
+          const int id = s_idx[t * TK + k];
+          if (id >= 0) {
+            const uint8_t* line = recs + int64_t(id) * kRecBytes + min((lane - 6 * i) * 128, kRecBytes - 16);
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
+          }
+        }
+      };
+      prefetch_tile(1);
       RecPart rec[kQuantRows];
 #pragma unroll
       for (int i = 0; i < kQuantRows; ++i) {
         const int k = pw + i * kQuantProducerWarps;
         if (n > 0 && k < TK) load_record(rec[i], recs, s_idx[k], lane, hi_off);
       }
+      if (q_late) q_part();  // now: the first score product waits for every warp's part
       for (int t = 0; t < n; ++t) {
-        if (t == NT - 1) {
-          if (q_late) q_part();
-          warp_wait(&aux->q_full, 0);
-        }
+        if (t == NT - 1) warp_wait(&aux->q_full, 0);
         if (t >= NT) warp_wait(&aux->empty[t % NT], ((t / NT) - 1) & 1);
         const uint32_t dst = sRing + (t % NT) * kTileBytes + lane_off;
+        prefetch_tile(t + 2);
 #pragma unroll
         for (int i = 0; i < kQuantRows; ++i) {
           const int k = pw + i * kQuantProducerWarps;
@@ -498,7 +522,6 @@ __global__ void __launch_bounds__(kQuant ? kQuantThreads : THREADS, 1)
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(smem_u32(&aux->full[t % NT]));
       }
-      if (n < NT && q_late) q_part();
     } else {
       for (int t = early_lead ? 1 : 0; t < n; ++t) {
         if (t == NT - 1) {
@@ -511,11 +534,11 @@ __global__ void __launch_bounds__(kQuant ? kQuantThreads : THREADS, 1)
       if (n < NT && q_late) q_part();
       cp_async_wait<0>();
     }
-  } else if (warp == kMmaWarp || warp == 12) {
+  } else if (warp == R::kPV0 || warp == R::kPV1) {
     // ------------------------------------------------------------ PV issuers
-    // warp 4: output dims 0-255 (O^T blocks 0, 1), warp 12: dims 256-511
+    // kPV0: output dims 0-255 (O^T blocks 0, 1), kPV1: dims 256-511
     if (q_late) q_part();
-    const int jb0 = warp == kMmaWarp ? 0 : 2;
+    const int jb0 = warp == R::kPV0 ? 0 : 2;
     if (lane == 0 && n > 0) {
       const uint32_t hi = tc::desc_hi(1024, tc::kLayoutSw128);
       const uint32_t v_lo = tc::desc_lo(sRing, kPairBytes);  // MN-major: LBO = the next 64 dims (next pair block)
@@ -711,7 +734,7 @@ __global__ void __launch_bounds__(kQuant ? kQuantThreads : THREADS, 1)
     if (n > 0) warp_wait(&aux->pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
     tc::fence_after_sync();
     if (tid == 0) SA_TRACE(kTrMisc, 2);
-  } else if (warp == 8) {
+  } else if (warp == R::kS) {
     // ------------------------------------------------------------ S issuer
     if (q_late) q_part();
     if (lane == 0 && n > 0) {
