@@ -75,7 +75,7 @@ struct Args {
   int B, Bt, groups, N, nkb, n_tiles, m_tiles;
   int split, rows_per;  // C CTAs an item; token rows each of them finishes
   int n_stages, tma_store;
-  uint32_t stage_bytes, part_off, recv_off, out_off, aux_off;
+  uint32_t stage_bytes, half_bytes, part_off, recv_off, out_off, aux_off;
   int32_t* status;
   long long wait_limit;
 };
@@ -95,7 +95,6 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
                    reinterpret_cast<uint64_t>(map)),
                "r"(src), "r"(x), "r"(y)
                : "memory");
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
 template <bool kF32>
@@ -106,17 +105,39 @@ __device__ __forceinline__ OutT<kF32> to_out(float v) {
   else return f2bf(v);
 }
 
-// CNT values of token rows [row, row + CNT) of the item's tile: staged at rows
-// [srow, ..) or stored to Y; rows from `rows` on are left out
+// Staging of a finished tile for the TMA store.  bf16: two halves of 64
+// columns, [row][128 B] with the 128-byte swizzle (what stmatrix and the
+// store take without bank conflicts); fp32: [row][128].
+template <bool kF32>
+__device__ __forceinline__ OutT<kF32>* stage_at(uint8_t* stage, uint32_t half_bytes, int row, int n) {
+  if constexpr (kF32) return reinterpret_cast<float*>(stage) + row * TILE_N + n;
+  else
+    return reinterpret_cast<__nv_bfloat16*>(stage + (n >> 6) * half_bytes + row * 128 +
+                                            ((((n >> 3) & 7) ^ (row & 7)) << 4)) + (n & 7);
+}
+
+// the staged tile's rows to Y[b0.., 128 t ..] (one thread)
+template <bool kF32>
+__device__ __forceinline__ void store_tile(const CUtensorMap* tm_y, uint32_t stage, uint32_t half_bytes, int t, int b0,
+                                           int N) {
+  if constexpr (kF32) {
+    tma_store_2d(tm_y, stage, t * TILE_N, b0);
+  } else {
+    tma_store_2d(tm_y, stage, t * TILE_N, b0);
+    if (t * TILE_N + 64 < N) tma_store_2d(tm_y, stage + half_bytes, t * TILE_N + 64, b0);
+  }
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+// CNT values of this thread's weight row, token rows [row, ..), to Y
 template <bool kF32, int CNT>
-__device__ __forceinline__ void put_rows(const Args& a, OutT<kF32>* stage, int srow, int nr, int64_t row, int rows,
-                                         int n, const float* v) {
-  if (a.tma_store) {
+__device__ __forceinline__ void store_rows(const Args& a, int64_t row, int rows, int n, const float* v) {
+  if (n >= a.N) return;
+  OutT<kF32>* o = static_cast<OutT<kF32>*>(a.y) + row * a.ld_y + n;
+  if (rows >= CNT) {  // no guard inside: the stores leave back to back
 #pragma unroll
-    for (int i = 0; i < CNT; ++i)
-      if (i < rows) stage[(srow + i) * TILE_N + nr] = to_out<kF32>(v[i]);
-  } else if (n < a.N) {
-    OutT<kF32>* o = static_cast<OutT<kF32>*>(a.y) + row * a.ld_y + n;
+    for (int i = 0; i < CNT; ++i) o[i * a.ld_y] = to_out<kF32>(v[i]);
+  } else {
 #pragma unroll
     for (int i = 0; i < CNT; ++i)
       if (i < rows) o[i * a.ld_y] = to_out<kF32>(v[i]);
@@ -244,7 +265,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
     const int quarter = warp & 3;        // TMEM lanes [32 quarter, 32 quarter + 32)
     const int nr = quarter * 32 + lane;  // this thread's row of the weight tile
     const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16);
-    OutT<kF32>* stage = reinterpret_cast<OutT<kF32>*>(smem + a.out_off);
+    uint8_t* stage = smem + a.out_off;
     const bool lead = tid == 64;
     if (lead && a.tma_store) tma::prefetch_map(&tm_y);
     if (C == 1) {
@@ -260,11 +281,45 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
         }
         tc::mbar_wait(smem_u32(&aux->acc_full[acc]), (li >> 1) & 1, a.status, 2, a.wait_limit);
         tc::fence_after_sync();
-        for (int c0 = 0; c0 < rows; c0 += 32) {
-          float v[32];
-          tc::tmem_ld32(trow + uint32_t(kMaxBt) * acc + c0, v);
-          tc::tmem_wait_ld();
-          put_rows<kF32, 32>(a, stage, c0, nr, b0 + c0, rows - c0, t * TILE_N + nr, v);
+        // rows past the tile's tokens are staged too (the store leaves them out)
+        const uint32_t tacc = trow + uint32_t(kMaxBt) * acc;
+        if (!kF32 && a.tma_store) {
+          // 16x256b fragments: thread i holds weight rows i / 4 and 8 + i / 4
+          // at tokens 2 (i % 4) + {0, 1}; stmatrix.trans turns 8x8 blocks
+          // around: four 16-byte pieces of token rows an instruction
+          // (element stores of the transposed tile took 200 cycles a row)
+          const int blk = lane >> 3, n0 = quarter * 32 + (blk & 1) * 8;
+          for (int c0 = 0; c0 < rows; c0 += 32) {
+            float v[2][16];
+            tc::tmem_ld16x256b_x4(tacc + c0, v[0]);
+            tc::tmem_ld16x256b_x4(tacc + (16u << 16) + c0, v[1]);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int r = 0; r < 4; r += 2) {
+                const uint32_t at = smem_u32(stage_at<false>(stage, a.half_bytes, c0 + 8 * (r + (blk >> 1)) + (lane & 7),
+                                                             n0 + 16 * h));
+                const float* p = v[h] + 4 * r;
+                asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at),
+                             "r"(pack_bf16x2(p[0], p[1])), "r"(pack_bf16x2(p[2], p[3])), "r"(pack_bf16x2(p[4], p[5])),
+                             "r"(pack_bf16x2(p[6], p[7]))
+                             : "memory");
+              }
+            }
+          }
+        } else {
+          for (int c0 = 0; c0 < rows; c0 += 32) {
+            float v[32];
+            tc::tmem_ld32(tacc + c0, v);
+            tc::tmem_wait_ld();
+            if (a.tma_store) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) *stage_at<kF32>(stage, a.half_bytes, c0 + i, nr) = to_out<kF32>(v[i]);
+            } else {
+              store_rows<kF32, 32>(a, b0 + c0, rows - c0, t * TILE_N + nr, v);
+            }
+          }
         }
         tc::fence_before_sync();
         __syncwarp();
@@ -272,7 +327,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
         if (a.tma_store) {
           tc::fence_proxy_async();
           tc::named_bar_sync(1, 128);
-          if (lead) tma_store_2d(&tm_y, smem_u32(stage), t * TILE_N, int(b0));
+          if (lead) store_tile<kF32>(&tm_y, smem_u32(stage), a.half_bytes, t, int(b0), a.N);
         }
       }
     } else {
@@ -294,8 +349,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
         tc::tmem_ld32(trow + c0, v);
         tc::tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (c0 + i < rows) part[(c0 + i) * TILE_N + nr] = v[i];
+        for (int i = 0; i < 32; ++i) part[(c0 + i) * TILE_N + nr] = v[i];  // (room for whole groups of 32)
       }
       tc::fence_proxy_async();  // the copy engine reads the partial
       tc::named_bar_sync(1, 128);
@@ -318,12 +372,17 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] += recv[(q * R + min(l0 + j, R - 1)) * TILE_N + nr];
         }
-        put_rows<kF32, 8>(a, stage, l0, nr, b0 + r0 + l0, own - l0, t * TILE_N + nr, v);
+        if (a.tma_store) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) *stage_at<kF32>(stage, a.half_bytes, l0 + j, nr) = to_out<kF32>(v[j]);
+        } else {
+          store_rows<kF32, 8>(a, b0 + r0 + l0, own - l0, t * TILE_N + nr, v);
+        }
       }
       if (a.tma_store && own > 0) {
         tc::fence_proxy_async();
         tc::named_bar_sync(1, 128);
-        if (lead) tma_store_2d(&tm_y, smem_u32(stage), t * TILE_N, int(b0) + r0);
+        if (lead) store_tile<kF32>(&tm_y, smem_u32(stage), a.half_bytes, t, int(b0) + r0, a.N);
       }
     }
     if (lead) lin::bulk_wait_read();  // the tiles have left shared memory
@@ -343,50 +402,47 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
   }
 }
 
-// X [B, K] -> codes [B, K/2] and scales in the product's order; the scales of
-// the last k-block past K are zero (their codes are zero-filled by the TMA).
+// X [B, K] -> codes [B, K/2] and scales in the product's order.  A warp takes
+// kQuantUnroll k-blocks of one token: its lanes hold the 256 elements of a
+// k-block, so the eight scales are two words of four (elements past K are
+// zero, and so is their scale).
 constexpr int kQuantThreads = 256;
-constexpr int kQuantUnroll = 2;
+constexpr int kQuantUnroll = 4;
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads) quant_x_kernel(const T* __restrict__ x, int64_t ld_x,
                                                                 uint32_t* __restrict__ codes,
-                                                                uint8_t* __restrict__ sf, int64_t total, int row_chunks,
-                                                                int Bt, int groups, int nkb) {
+                                                                uint8_t* __restrict__ sf, int B, int K, int Bt,
+                                                                int groups, int nkb) {
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t step = int64_t(gridDim.x) * kQuantThreads * kQuantUnroll;
-  for (int64_t c0 = int64_t(blockIdx.x) * kQuantThreads * kQuantUnroll; c0 < total; c0 += step) {
+  const int lane = threadIdx.x & 31;
+  const int runs = (nkb + kQuantUnroll - 1) / kQuantUnroll;  // of a token
+  const int64_t total = int64_t(B) * runs, step = int64_t(gridDim.x) * (kQuantThreads / 32);
+  for (int64_t w = int64_t(blockIdx.x) * (kQuantThreads / 32) + (threadIdx.x >> 5); w < total; w += step) {
+    const int b = int(w / runs), kb0 = int(w - int64_t(b) * runs) * kQuantUnroll;
+    const T* src = x + b * ld_x;
     float v[kQuantUnroll][mx::kVec];
-    int64_t at[kQuantUnroll];
-    int row[kQuantUnroll], col[kQuantUnroll];
 #pragma unroll
     for (int u = 0; u < kQuantUnroll; ++u) {
-      at[u] = c0 + u * kQuantThreads + threadIdx.x;
-      row[u] = col[u] = 0;
+      const int k = (kb0 + u) * KBW + lane * mx::kVec;
 #pragma unroll
       for (int i = 0; i < mx::kVec; ++i) v[u][i] = 0.f;
-      if (at[u] < total) {
-        row[u] = int(at[u] / row_chunks);
-        col[u] = int(at[u] - int64_t(row[u]) * row_chunks);
-        mx::load8(x + row[u] * ld_x + int64_t(col[u]) * mx::kVec, v[u]);
-      }
+      if (k < K) mx::load8(src + k, v[u]);
     }
+    const int mt = b / Bt, r = b - mt * Bt;
+    uint8_t* row_sf = sf + (int64_t(mt) * nkb * groups + (r >> 7)) * kSfBytes + (r & 31) * 16 + ((r >> 5) & 3) * 4;
 #pragma unroll
     for (int u = 0; u < kQuantUnroll; ++u) {
+      const int kb = kb0 + u, k = kb * KBW + lane * mx::kVec;
       const uint32_t sc = mx::scale_code(v[u]);
-      if (at[u] >= total) continue;
-      codes[at[u]] = mx::codes8(v[u], sc);
-      if ((col[u] & 3) == 0) {
-        const int mt = row[u] / Bt, r = row[u] - mt * Bt;
-        int i = col[u] >> 2;  // the block's number along K
-        const bool last = col[u] + 4 == row_chunks;
-        do {
-          const int kb = i / kSfPerKb, j = i % kSfPerKb;
-          sf[((int64_t(mt) * nkb + kb) * groups + (r >> 7)) * kSfBytes + (j >> 2) * 512 + (r & 31) * 16 +
-             ((r >> 5) & 3) * 4 + (j & 3)] = uint8_t(i == (col[u] >> 2) ? sc : 0u);
-          ++i;
-        } while (last && i < nkb * kSfPerKb);
-      }
+      if (k < K) codes[(int64_t(b) * K + k) / mx::kVec] = mx::codes8(v[u], sc);
+      // blocks 4 j .. 4 j + 3 of the k-block, from lanes 16 j + {0, 4, 8, 12}
+      uint32_t word = sc;
+      word |= __shfl_down_sync(0xffffffffu, sc, 4) << 8;
+      word |= __shfl_down_sync(0xffffffffu, sc, 8) << 16;
+      word |= __shfl_down_sync(0xffffffffu, sc, 12) << 24;
+      if ((lane & 15) == 0 && kb < nkb)
+        *reinterpret_cast<uint32_t*>(row_sf + int64_t(kb) * groups * kSfBytes + (lane >> 4) * 512) = word;
     }
   }
 }
@@ -473,20 +529,24 @@ struct Plan {
 static int lay_out(const Plan& p, int B, int es, bool tma_store, Args* a) {
   const int tokens = std::min(B, p.Bt);
   const int R = (tokens + p.split - 1) / p.split;
-  const int out_rows = p.split > 1 ? R : p.Bt;
+  // whole groups of rows as the epilogue writes them: 32, a split's owner 8
+  const int out_rows = p.split > 1 ? (R + 7) / 8 * 8 : (p.Bt + 31) / 32 * 32;
   const uint32_t stage = uint32_t(kWBytes + p.Bt * (KBW / 2) + p.groups * kSfBytes);
   const uint32_t out_bytes = tma_store ? (uint32_t(out_rows) * TILE_N * es + 1023u) & ~1023u : 0u;
-  const uint32_t part = p.split > 1 ? uint32_t(tokens) * TILE_N * 4 : 0u;
+  const uint32_t part = p.split > 1 ? uint32_t((tokens + 31) / 32 * 32) * TILE_N * 4 : 0u;
   const uint32_t recv = p.split > 1 ? uint32_t(p.split * R) * TILE_N * 4 : 0u;
   const uint32_t room = kSmemBytes - 1024 - kAuxBytes;
   if (out_bytes >= room || part + recv + out_bytes > room) return 0;
   const int stages = std::min<int>(kMaxStages, (room - out_bytes) / stage);
   if (stages < 2) return 0;
-  const uint32_t ring = std::max(stages * stage, part + recv);  // the partials take the ring's place
+  // the partials take the ring's place; the staged tile starts on 1024 B
+  const uint32_t ring = (std::max(stages * stage, part + recv) + 1023u) & ~1023u;
+  if (ring + out_bytes > room) return 0;
   if (a) {
     a->n_stages = stages;
     a->stage_bytes = stage;
     a->rows_per = R;
+    a->half_bytes = uint32_t(out_rows) * 128;
     a->part_off = 0;
     a->recv_off = part;
     a->out_off = ring;
@@ -625,22 +685,23 @@ extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const v
     tma::EncodeTiledFn fn = tma::encode_fn();
     const cuuint64_t dims[2] = {uint64_t(N), uint64_t(B)};
     const cuuint64_t strides[1] = {uint64_t(B == 1 ? N : ld_y) * es};
-    const cuuint32_t box[2] = {uint32_t(lmx::TILE_N), uint32_t(p.split > 1 ? a.rows_per : p.Bt)};
+    const cuuint32_t box[2] = {uint32_t(out_f32 ? lmx::TILE_N : 64), uint32_t(p.split > 1 ? a.rows_per : p.Bt)};
     const cuuint32_t estr[2] = {1, 1};
     if (!fn || fn(&tm_y, out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, y, dims,
-                  strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                  strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  out_f32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
       set_error("linear_mxfp4: cuTensorMapEncodeTiled (Y) failed");
       return DSA_ERR_CUDA;
     }
   }
-  const int64_t total = int64_t(B) * (K / mx::kVec);
-  const int per = lmx::kQuantThreads * lmx::kQuantUnroll;
-  const dim3 qgrid(unsigned(std::min<int64_t>((total + per - 1) / per, int64_t(num_sms()) * 16)));
+  const int64_t q_warps = int64_t(B) * ((nkb + lmx::kQuantUnroll - 1) / lmx::kQuantUnroll);
+  const int per = lmx::kQuantThreads / 32;
+  const dim3 qgrid(unsigned(std::min<int64_t>((q_warps + per - 1) / per, int64_t(num_sms()) * 32)));
   auto quant = [&](auto* ptr) {
     using T = std::remove_pointer_t<decltype(ptr)>;
     launch_pdl(lmx::quant_x_kernel<T>, qgrid, dim3(lmx::kQuantThreads), 0, st, static_cast<const T*>(x), ld_x,
-               reinterpret_cast<uint32_t*>(codes), sf, total, K / mx::kVec, p.Bt, p.groups, nkb);
+               reinterpret_cast<uint32_t*>(codes), sf, B, K, p.Bt, p.groups, nkb);
   };
   if (x_type == DSA_BF16)
     quant(static_cast<__nv_bfloat16*>(nullptr));
