@@ -164,8 +164,8 @@ def test_linear_mxfp4_refusals():
     assert L.dsa_linear_mxfp4_packed_bytes(128, 48) == 0 and L.dsa_linear_mxfp4_packed_bytes(0, 64) == 0
     assert L.dsa_linear_mxfp4_packed_bytes(1 << 25, 64) == 0
     assert L.dsa_linear_mxfp4_workspace_size(0, 64, 64) == 0 and L.dsa_linear_mxfp4_workspace_size(4, 64, 48) == 0
-    # codes of 4 tokens rounded up to 256 B, scales of one k-block for one group of 128 tokens
-    assert L.dsa_linear_mxfp4_workspace_size(4, 64, 64) == 256 + 1024
+    # one k-block of 32 token rows of codes and the scales of one group of 128 tokens
+    assert L.dsa_linear_mxfp4_workspace_size(4, 64, 64) == 32 * 128 + 1024
     p = L.dsa_linear_mxfp4_pack
     _refused(p(None, 16, 128, 256, 16, 17408, None), "null")
     _refused(p(16, 16, 128, 250, 16, 17408, None), "multiple of 32")

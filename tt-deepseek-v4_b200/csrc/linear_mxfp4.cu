@@ -5,9 +5,8 @@
 // block scales in the tensor cores: products of E2M1 values are exact and no
 // operand is expanded.
 //
-// Two launches: X's quantisation (codes [B, K/2] and block scales in the
-// order the tensor cores take them), then the product, whose weight loads
-// start before the first has ended.
+// Two launches: X's quantisation into tiles of the weight's layout, then the
+// product, whose weight loads start before the first has ended.
 //
 // Weight layout (dsa_linear_mxfp4_pack, once at load time): per (128-row tile
 // t, 256-wide k-block kb) 17 KB: the codes of the 128 rows as a 128-byte
@@ -16,19 +15,25 @@
 // four (byte (r % 32) * 16 + (r / 32) * 4 + j), zero past N and K.  A CTA's
 // k-range is one contiguous run of memory that it reads with 17 KB bulk copies.
 //
+// X's scratch holds the same tiles with Bt token rows: codes, then 1 KB of
+// scales for each 128 tokens.
+//
 // A work item is (128 weight rows, Bt <= 192 tokens):
-//   warp 0      producer: per k-block the weight tile (bulk copy), the
-//               [Bt x 256] codes of X (2-D TMA) and their scales (bulk copy)
-//               into a ring;
-//   warp 1      MMA issuer: scales from shared into tensor memory
-//               (tcgen05.cp), then Y^T = W . X^T, M = 128 weight rows,
-//               N = Bt tokens, K = 64 a step, into one of two accumulators:
-//               the epilogue of item i overlaps item i + 1;
-//   warps 2-5   epilogue, thread = weight row: rounding, a staging tile
-//               [token][128] and a TMA store (element stores where Y's rows
-//               are not 16-byte aligned).
-// Tensor memory: 2 x 192 accumulator columns and 2 x 24 of scales (8 for W, 16
-// for X a k-block).
+//   warp 0      producer: per k-block two bulk copies, a weight tile and an X
+//               tile, into a ring;
+//   warp 6      scales from shared into tensor memory (tcgen05.cp), a set of
+//               columns for each stage of the ring;
+//   warp 1      MMA issuer: Y^T = W . X^T, M = 128 weight rows, N = Bt
+//               tokens, K = 64 a step, into one of two accumulators: the
+//               epilogue of item i overlaps item i + 1;
+//   warps 2-5   epilogue, thread = weight row: rounding, a staging tile and a
+//               TMA store (element stores where Y's rows are not 16-byte
+//               aligned).
+// One thread issued copies of scales and products at first: a tcgen05.cp
+// costs its issuer ~100 cycles, so a k-block took 1400 cycles against ~400 of
+// MMA time (4096 x 4096 x 8192: 128 us).
+// Tensor memory: 2 x 192 accumulator columns, 128 of scales (8 a stage for W, 8
+// for each 128 tokens of X).
 //
 // Few items (decode): the C CTAs of a cluster share an item, each over its
 // own part of K.  After the last product a cluster barrier frees every ring;
@@ -56,20 +61,23 @@ constexpr int kCodeBytes = TILE_N * KBW / 2;    // 16 KB
 constexpr int kSfBytes = TILE_N * kSfPerKb;     // 1 KB for each 128 rows
 constexpr int kWBytes = kCodeBytes + kSfBytes;  // a weight tile
 constexpr int kMaxBt = 192;
-constexpr int kMaxStages = 12;
+constexpr int kMaxStages = 8;
 constexpr int kMaxSplit = 16;
-constexpr int THREADS = 192;
+constexpr int THREADS = 224;
 constexpr int kSmemBytes = 232448;
 constexpr int kAuxBytes = 256;
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColSf = 2 * kMaxBt;         // scales: per parity 8 columns of W, 16 of X
-constexpr uint32_t kSfCols = 24;
-static_assert(kColSf + 2 * kSfCols <= kTmemCols, "TMEM columns");
+constexpr uint32_t kColSf = 2 * kMaxBt;         // scales of each stage: 8 columns of W, 8 a group of X
+__host__ __device__ constexpr int sf_cols(int groups) { return 8 + 8 * groups; }
+__host__ __device__ constexpr int max_stages(int groups) {
+  return (int(kTmemCols) - int(kColSf)) / sf_cols(groups) < kMaxStages ? (int(kTmemCols) - int(kColSf)) / sf_cols(groups)
+                                                                       : kMaxStages;
+}
 static_assert(kWBytes % 1024 == 0, "the swizzled operands start on 1024 B");
 
 struct Args {
   const uint8_t* w;
-  const uint8_t* xsf;   // X's scales: [m tile][k-block][groups of 128 tokens] of 1 KB
+  const uint8_t* x;     // X's tiles [m tile][k-block]
   void* y;
   int64_t ld_y;
   int B, Bt, groups, N, nkb, n_tiles, m_tiles;
@@ -83,6 +91,7 @@ struct Args {
 struct Aux {
   uint64_t full[kMaxStages];
   uint64_t empty[kMaxStages];
+  uint64_t sf_full[kMaxStages];
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
   uint64_t ready;
@@ -146,7 +155,6 @@ __device__ __forceinline__ void store_rows(const Args& a, int64_t row, int rows,
 
 template <bool kF32>
 __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
-                                                                  const __grid_constant__ CUtensorMap tm_x,
                                                                   const __grid_constant__ CUtensorMap tm_y) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -159,8 +167,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
   const int n_items = a.n_tiles * a.m_tiles;
   const int kb0 = rank * a.nkb / C, kb1 = (rank + 1) * a.nkb / C;
   const int NS = a.n_stages;
-  const uint32_t x_bytes = uint32_t(a.Bt) * (KBW / 2), xsf_bytes = uint32_t(a.groups) * kSfBytes;
-  const uint32_t stage_tx = kWBytes + x_bytes + xsf_bytes;
+  const uint32_t x_bytes = uint32_t(a.Bt) * (KBW / 2);
+  const uint32_t x_tile = x_bytes + uint32_t(a.groups) * kSfBytes;
+  const uint32_t stage_tx = kWBytes + x_tile;
 
   if (warp == 1) {
     tc::tmem_alloc(smem_u32(&aux->tmem_base), kTmemCols);
@@ -170,6 +179,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
     for (int s = 0; s < NS; ++s) {
       tc::mbar_init(smem_u32(&aux->full[s]), 1);
       tc::mbar_init(smem_u32(&aux->empty[s]), 1);
+      tc::mbar_init(smem_u32(&aux->sf_full[s]), 1);
     }
     for (int s = 0; s < 2; ++s) {
       tc::mbar_init(smem_u32(&aux->acc_full[s]), 1);
@@ -199,27 +209,30 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
   pdl_wait();
   pdl_launch_dependents();
 
+  // a stage's address, barrier and parity advance by counters: a division a
+  // k-block showed in the issuers' time
   if (warp == 0) {
     // ---------------------------------------------------------------- producer
     if (lane == 0) {
-      tma::prefetch_map(&tm_x);
-      int it = 0;
+      int it = 0, s = 0;
+      uint32_t ph = 1;  // parity of the stage's last release
       for (int item = cid; item < n_items; item += n_cl) {
         const int t = item / a.m_tiles, mt = item - t * a.m_tiles;
         const uint8_t* wt = a.w + (int64_t(t) * a.nkb + kb0) * kWBytes;
-        const uint8_t* xs = a.xsf + (int64_t(mt) * a.nkb + kb0) * xsf_bytes;
-        for (int kb = kb0; kb < kb1; ++kb, ++it, wt += kWBytes, xs += xsf_bytes) {
-          const int s = it % NS;
+        const uint8_t* xt = a.x + (int64_t(mt) * a.nkb + kb0) * x_tile;
+        for (int kb = kb0; kb < kb1; ++kb, ++it, wt += kWBytes, xt += x_tile) {
           const uint32_t st = sbase + s * a.stage_bytes;
           const uint32_t fb = smem_u32(&aux->full[s]);
           if (it >= npre) {
-            if (it >= NS) tc::mbar_wait(smem_u32(&aux->empty[s]), ((it / NS) - 1) & 1, a.status, 2, a.wait_limit);
+            if (it >= NS) tc::mbar_wait(smem_u32(&aux->empty[s]), ph, a.status, 2, a.wait_limit);
             tma::mbar_arrive_expect_tx(fb, stage_tx);
             lin::bulk_load(st, wt, kWBytes, fb);
           }
-          // (the map's columns are pairs of codes: 64 two-byte words a k-block)
-          tma::load_2d(st + kWBytes, &tm_x, kb * (KBW / 4), mt * a.Bt, fb);
-          lin::bulk_load(st + kWBytes + x_bytes, xs, xsf_bytes, fb);
+          lin::bulk_load(st + kWBytes, xt, x_tile, fb);
+          if (++s == NS) {
+            s = 0;
+            ph ^= 1;
+          }
         }
       }
     }
@@ -228,39 +241,75 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
     // ---------------------------------------------------------------- MMA issuer
     if (lane == 0) {
       const uint32_t id0 = tc::idesc_mxf4(128, a.Bt, 0), id2 = tc::idesc_mxf4(128, a.Bt, 2);
-      int it = 0, li = 0;
+      const uint32_t hi = tc::desc_hi(1024, tc::kLayoutSw128);
+      const uint32_t sf_step = sf_cols(a.groups), sfb_step = 4 * a.groups;
+      int s = 0, li = 0;
+      uint32_t ph = 0;
       for (int item = cid; item < n_items; item += n_cl, ++li) {
         const int acc = li & 1;
         if (li >= 2) tc::mbar_wait(smem_u32(&aux->acc_empty[acc]), ((li - 2) >> 1) & 1, a.status, 2, a.wait_limit);
         tc::fence_after_sync();
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % NS;
-          tc::mbar_wait(smem_u32(&aux->full[s]), (it / NS) & 1, a.status, 2, a.wait_limit);
-          tc::fence_after_sync();
+        const uint32_t d = tmem + uint32_t(kMaxBt) * acc;
+        for (int kb = kb0; kb < kb1; ++kb) {
           const uint32_t st = sbase + s * a.stage_bytes;
-          const uint32_t sx = st + kWBytes + x_bytes;
-          const uint32_t sfa = tmem + kColSf + kSfCols * (it & 1), sfb = sfa + 8;
+          const uint32_t sfa = tmem + kColSf + sf_step * s, sfb = sfa + 8;
+          const uint32_t a_lo = tc::desc_lo(st, 16), b_lo = tc::desc_lo(st + kWBytes, 16);
+          tc::mbar_wait(smem_u32(&aux->full[s]), ph, a.status, 2, a.wait_limit);
+          tc::mbar_wait(smem_u32(&aux->sf_full[s]), ph, a.status, 2, a.wait_limit);
+          tc::fence_after_sync();
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            tc::cp_scales(sfa + 4 * j, st + kCodeBytes + 512 * j);
-            for (int g = 0; g < a.groups; ++g) tc::cp_scales(sfb + 8 * j + 4 * g, sx + g * kSfBytes + 512 * j);
-          }
-#pragma unroll
-          for (int ks = 0; ks < KBW / 64; ++ks) {
-            const uint64_t ad = tc::smem_desc(st + ks * 32, 16, 1024, tc::kLayoutSw128);
-            const uint64_t bd = tc::smem_desc(st + kWBytes + ks * 32, 16, 1024, tc::kLayoutSw128);
-            tc::mma_mxf4(tmem + uint32_t(kMaxBt) * acc, ad, bd, (ks & 1) ? id2 : id0, sfa + 4 * (ks >> 1),
-                         sfb + 8 * (ks >> 1), (kb > kb0 || ks) ? 1u : 0u);
-          }
+          for (int ks = 0; ks < KBW / 64; ++ks)
+            tc::mma_mxf4(d, tc::desc_pack(a_lo + ks * 2, hi), tc::desc_pack(b_lo + ks * 2, hi), (ks & 1) ? id2 : id0,
+                         sfa + 4 * (ks >> 1), sfb + sfb_step * (ks >> 1), (kb > kb0 || ks) ? 1u : 0u);
           tc::mma_commit(smem_u32(&aux->empty[s]));
+          if (++s == NS) {
+            s = 0;
+            ph ^= 1;
+          }
         }
         tc::mma_commit(smem_u32(&aux->acc_full[acc]));
       }
     }
     __syncwarp();
+  } else if (warp == 6) {
+    // ---------------------------------------------------------------- scales
+    // A stage's columns are free once its MMAs have completed, which is when
+    // the producer refills the stage: the wait for `full` covers both.
+    if (lane == 0) {
+      const uint32_t hi = tc::desc_hi(128, tc::kLayoutNone);
+      const uint32_t sf_step = sf_cols(a.groups);
+      int s = 0;
+      uint32_t ph = 0;
+      for (int item = cid; item < n_items; item += n_cl) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          const uint32_t st = sbase + s * a.stage_bytes;
+          const uint32_t sfa = tmem + kColSf + sf_step * s;
+          const uint32_t w_lo = tc::desc_lo(st + kCodeBytes, 16), x_lo = tc::desc_lo(st + kWBytes + x_bytes, 16);
+          tc::mbar_wait(smem_u32(&aux->full[s]), ph, a.status, 2, a.wait_limit);
+          tc::fence_after_sync();
+          tc::cp_scales(sfa, tc::desc_pack(w_lo, hi));
+          tc::cp_scales(sfa + 4, tc::desc_pack(w_lo + 32, hi));
+          if (a.groups == 1) {
+            tc::cp_scales(sfa + 8, tc::desc_pack(x_lo, hi));
+            tc::cp_scales(sfa + 12, tc::desc_pack(x_lo + 32, hi));
+          } else {
+            tc::cp_scales(sfa + 8, tc::desc_pack(x_lo, hi));
+            tc::cp_scales(sfa + 12, tc::desc_pack(x_lo + 64, hi));
+            tc::cp_scales(sfa + 16, tc::desc_pack(x_lo + 32, hi));
+            tc::cp_scales(sfa + 20, tc::desc_pack(x_lo + 96, hi));
+          }
+          tc::mma_commit(smem_u32(&aux->sf_full[s]));
+          if (++s == NS) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+    __syncwarp();
   }
 
-  if (warp >= 2) {
+  if (warp >= 2 && warp <= 5) {
     // ---------------------------------------------------------------- epilogue (warps 2-5)
     const int quarter = warp & 3;        // TMEM lanes [32 quarter, 32 quarter + 32)
     const int nr = quarter * 32 + lane;  // this thread's row of the weight tile
@@ -402,16 +451,14 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
   }
 }
 
-// X [B, K] -> codes [B, K/2] and scales in the product's order.  A warp takes
-// kQuantUnroll k-blocks of one token: its lanes hold the 256 elements of a
-// k-block, so the eight scales are two words of four (elements past K are
-// zero, and so is their scale).
+// X [B, K] -> its tiles.  A warp takes kQuantUnroll k-blocks of one token: its
+// lanes hold the 256 elements of a k-block, so it writes the row's 128 B of
+// codes and two words of four scales (past K: zeros).
 constexpr int kQuantThreads = 256;
 constexpr int kQuantUnroll = 4;
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads) quant_x_kernel(const T* __restrict__ x, int64_t ld_x,
-                                                                uint32_t* __restrict__ codes,
-                                                                uint8_t* __restrict__ sf, int B, int K, int Bt,
+                                                                uint8_t* __restrict__ tiles, int B, int K, int Bt,
                                                                 int groups, int nkb) {
   pdl_wait();
   pdl_launch_dependents();
@@ -430,19 +477,22 @@ __global__ void __launch_bounds__(kQuantThreads) quant_x_kernel(const T* __restr
       if (k < K) mx::load8(src + k, v[u]);
     }
     const int mt = b / Bt, r = b - mt * Bt;
-    uint8_t* row_sf = sf + (int64_t(mt) * nkb * groups + (r >> 7)) * kSfBytes + (r & 31) * 16 + ((r >> 5) & 3) * 4;
+    const int tile_bytes = Bt * (KBW / 2) + groups * kSfBytes;
+    uint8_t* tile = tiles + (int64_t(mt) * nkb + kb0) * tile_bytes;
+    const int at_code = r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
+    const int at_sf = Bt * (KBW / 2) + (r >> 7) * kSfBytes + (lane >> 4) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4;
 #pragma unroll
     for (int u = 0; u < kQuantUnroll; ++u) {
-      const int kb = kb0 + u, k = kb * KBW + lane * mx::kVec;
       const uint32_t sc = mx::scale_code(v[u]);
-      if (k < K) codes[(int64_t(b) * K + k) / mx::kVec] = mx::codes8(v[u], sc);
       // blocks 4 j .. 4 j + 3 of the k-block, from lanes 16 j + {0, 4, 8, 12}
       uint32_t word = sc;
       word |= __shfl_down_sync(0xffffffffu, sc, 4) << 8;
       word |= __shfl_down_sync(0xffffffffu, sc, 8) << 16;
       word |= __shfl_down_sync(0xffffffffu, sc, 12) << 24;
-      if ((lane & 15) == 0 && kb < nkb)
-        *reinterpret_cast<uint32_t*>(row_sf + int64_t(kb) * groups * kSfBytes + (lane >> 4) * 512) = word;
+      if (kb0 + u < nkb) {
+        *reinterpret_cast<uint32_t*>(tile + u * tile_bytes + at_code) = mx::codes8(v[u], sc);
+        if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(tile + u * tile_bytes + at_sf) = word;
+      }
     }
   }
 }
@@ -537,7 +587,7 @@ static int lay_out(const Plan& p, int B, int es, bool tma_store, Args* a) {
   const uint32_t recv = p.split > 1 ? uint32_t(p.split * R) * TILE_N * 4 : 0u;
   const uint32_t room = kSmemBytes - 1024 - kAuxBytes;
   if (out_bytes >= room || part + recv + out_bytes > room) return 0;
-  const int stages = std::min<int>(kMaxStages, (room - out_bytes) / stage);
+  const int stages = std::min<int>(max_stages(p.groups), (room - out_bytes) / stage);
   if (stages < 2) return 0;
   // the partials take the ring's place; the staged tile starts on 1024 B
   const uint32_t ring = (std::max(stages * stage, part + recv) + 1023u) & ~1023u;
@@ -587,7 +637,9 @@ static Plan pick_plan(int B, int N, int nkb) {
   return best;
 }
 
-static int64_t code_bytes(int64_t B, int64_t K) { return (B * (K / 2) + 255) / 256 * 256; }
+static size_t x_bytes_for(const Plan& p, int nkb) {
+  return size_t(p.m_tiles) * nkb * (p.Bt * (KBW / 2) + p.groups * kSfBytes);
+}
 static int n_kblocks(int K) { return (K + KBW - 1) / KBW; }
 static bool good_sizes(int64_t B, int64_t N, int64_t K) {
   return B >= 0 && B <= (1 << 24) && N > 0 && N <= (1 << 24) && K > 0 && K <= (1 << 24) && K % mx::kBlock == 0;
@@ -623,7 +675,7 @@ extern "C" size_t dsa_linear_mxfp4_workspace_size(int B, int N, int K) {
   if (!lmx::good_sizes(B, N, K) || B == 0) return 0;
   const int nkb = lmx::n_kblocks(K);
   const lmx::Plan p = lmx::pick_plan(B, N, nkb);
-  return size_t(lmx::code_bytes(B, K)) + size_t(p.m_tiles) * nkb * p.groups * lmx::kSfBytes;
+  return lmx::x_bytes_for(p, nkb);
 }
 
 extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const void* w_packed, void* y, int64_t ld_y,
@@ -641,19 +693,17 @@ extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const v
   if (B == 0) return DSA_OK;
   const int nkb = lmx::n_kblocks(K);
   const lmx::Plan p = lmx::pick_plan(B, N, nkb);
-  const int64_t cb = lmx::code_bytes(B, K);
-  const size_t need = size_t(cb) + size_t(p.m_tiles) * nkb * p.groups * lmx::kSfBytes;
+  const size_t need = lmx::x_bytes_for(p, nkb);
   if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)) {
     set_error("linear_mxfp4: needs %zu bytes of 16-byte aligned workspace (got %zu)", need, workspace_bytes);
     return DSA_ERR_WORKSPACE;
   }
-  uint8_t* codes = static_cast<uint8_t*>(workspace);
-  uint8_t* sf = codes + cb;
+  uint8_t* tiles = static_cast<uint8_t*>(workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 
   lmx::Args a{};
   a.w = static_cast<const uint8_t*>(w_packed);
-  a.xsf = sf;
+  a.x = tiles;
   a.y = y;
   a.ld_y = ld_y;
   a.B = B;
@@ -674,13 +724,8 @@ extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const v
     set_error("linear_mxfp4: no launch configuration fits");
     return DSA_ERR_CUDA;
   }
-  CUtensorMap tm_x, tm_y;
+  CUtensorMap tm_y;
   memset(&tm_y, 0, sizeof(tm_y));
-  // codes as [B, K/4] two-byte words
-  if (!tma::make_2d_bf16(&tm_x, codes, uint64_t(K) / 4, uint64_t(B), uint64_t(K) / 2, 64, uint32_t(p.Bt))) {
-    set_error("linear_mxfp4: cuTensorMapEncodeTiled failed");
-    return DSA_ERR_CUDA;
-  }
   if (a.tma_store) {
     tma::EncodeTiledFn fn = tma::encode_fn();
     const cuuint64_t dims[2] = {uint64_t(N), uint64_t(B)};
@@ -701,7 +746,7 @@ extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const v
   auto quant = [&](auto* ptr) {
     using T = std::remove_pointer_t<decltype(ptr)>;
     launch_pdl(lmx::quant_x_kernel<T>, qgrid, dim3(lmx::kQuantThreads), 0, st, static_cast<const T*>(x), ld_x,
-               reinterpret_cast<uint32_t*>(codes), sf, B, K, p.Bt, p.groups, nkb);
+               tiles, B, K, p.Bt, p.groups, nkb);
   };
   if (x_type == DSA_BF16)
     quant(static_cast<__nv_bfloat16*>(nullptr));
@@ -725,7 +770,7 @@ extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const v
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.split > 1 ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, out_f32 ? lmx::linear_mxfp4_kernel<true> : lmx::linear_mxfp4_kernel<false>, a, tm_x, tm_y);
+  cudaLaunchKernelEx(&cfg, out_f32 ? lmx::linear_mxfp4_kernel<true> : lmx::linear_mxfp4_kernel<false>, a, tm_y);
   DSA_CHECK_LAUNCH("linear_mxfp4");
   return DSA_OK;
 }

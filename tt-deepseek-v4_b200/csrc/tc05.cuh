@@ -103,10 +103,9 @@ __device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint6
 }
 // 32 rows of 16 B in shared memory (8x16-B core matrices, 128 B apart) into
 // four columns of tensor memory, the same for each of the four 32-lane
-// sub-partitions; ordered before the tcgen05.mma this thread issues next
-__device__ __forceinline__ void cp_scales(uint32_t tmem, uint32_t saddr) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem),
-               "l"(smem_desc(saddr, 16, 128, kLayoutNone)));
+// sub-partitions (descriptor: no swizzle, stride 128 B)
+__device__ __forceinline__ void cp_scales(uint32_t tmem, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc));
 }
 
 // arrive on an mbarrier once all previously issued tcgen05.mma of this thread complete
