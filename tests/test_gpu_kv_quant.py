@@ -84,6 +84,27 @@ def test_write_is_the_oracles_act_quant(cuda_dev, B, S, D, rope, win, offset, ex
     assert torch.equal(cache.cpu(), want)
 
 
+@pytest.mark.parametrize("amax", [448.0, 447.0, 1.0, 3.0, 1e-4, 5e-5, 0.7109375, 3.3e38, 1.1e-38, 2.0 ** -100, 96.5])
+def test_write_of_every_bf16_value(cuda_dev, amax):
+    """Every bf16 number up to amax, in blocks of that maximum: the quotient
+    is the correctly rounded one, so the codes are the oracle's."""
+    from dsv4attn import ops
+    x = torch.arange(0x7f80, dtype=torch.int32).to(torch.int16).view(BF)
+    top = torch.tensor([amax]).to(BF)
+    x = torch.cat([x[x < top], -x[x < top]])
+    x = torch.cat([x, torch.zeros(-x.numel() % 63, dtype=BF)]).view(-1, 63)
+    x = torch.cat([x, top.expand(x.shape[0], 1)], 1)
+    x = torch.cat([x, torch.zeros(-x.shape[0] % 8, 64, dtype=BF)])
+    kv = x.view(1, -1, 512)
+    n = kv.shape[1]
+    cache = ops.kv_quant_cache(1, n, 512, 0, device=cuda_dev)
+    ops.kv_quant_write(kv.to(cuda_dev), cache, torch.zeros(1, dtype=I32, device=cuda_dev), n, rope_dim=0)
+    codes, s, _ = _want_rows(kv, 0)
+    got, _, gs = ops.kv_quant_views(cache, 512, 0)
+    assert torch.equal(gs.cpu().view(-1), s.view(-1))
+    assert torch.equal(got.cpu().view(U8).view(-1), codes.view(U8).view(-1))
+
+
 def test_write_error_is_half_a_step(cuda_dev):
     """|value - x| <= |x| 2^-4 (half an e4m3 step) or half of the smallest
     step, s 2^-10, then bf16's 2^-8; s and the quotient are fp32: 3 roundings
