@@ -257,18 +257,18 @@ def linear_mxfp4(x: torch.Tensor, w: MXFP4Weight, out: torch.Tensor | None = Non
         raise ValueError(f"x must be [B, {K}] with contiguous rows, got {tuple(x.shape)}")
     B = x.shape[0]
     dtype = F32 if out_f32 else BF16
+    stream = _launch_stream(x, w.packed, out, status)
     if out is None:
-        out = x.new_empty((B, N), dtype=dtype)
+        out = torch.empty((B, N), dtype=dtype, device=x.device)
     else:
         _need(out, "out", dtype)
         if out.dim() != 2 or out.shape[0] != B or out.shape[1] < N or out.stride(1) != 1:
             raise ValueError(f"out must be [{B}, >={N}] with contiguous rows, got {tuple(out.shape)}")
-    stream = _launch_stream(x, w.packed, out, status)
     if B == 0:
         return out
     L = lib()
     need = L.dsa_linear_mxfp4_workspace_size(B, N, K)
-    buf = ws.get(need) if ws is not None else x.new_empty(need, dtype=torch.uint8)
+    buf = ws.get(need) if ws is not None else torch.empty(need, dtype=_U8, device=x.device)
     check(L.dsa_linear_mxfp4(x.data_ptr(), x_type, x.stride(0), w.packed.data_ptr(), out.data_ptr(), out.stride(0),
                              B, N, K, out_f32, buf.data_ptr(), need, _ptr(status), stream), "linear_mxfp4")
     return out
@@ -304,6 +304,7 @@ def act_quant_block(x: torch.Tensor, block: int = 64, fp8_max: float = 448.0, ep
 
 
 _X_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_U8 = torch.uint8
 
 
 def _row_stride(t: torch.Tensor, name: str) -> int:
@@ -324,12 +325,11 @@ def _launch_stream(t: torch.Tensor, *others) -> int:
     """The current stream of t's device.  Launches go to the current device:
     t and the other tensors must be on it."""
     dev = t.get_device()
-    cur = torch.cuda.current_device()
     for o in others:
         if o is not None and o.get_device() != dev:
             raise ValueError(f"tensors on {t.device} and {o.device}")
-    if dev != cur:
-        raise ValueError(f"tensor on {t.device}, current device is cuda:{cur}")
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"tensor on {t.device}, current device is cuda:{torch.cuda.current_device()}")
     return _raw_stream(dev)
 
 
@@ -355,27 +355,28 @@ def mxfp4_quant(x: torch.Tensor, out=None, codes: torch.Tensor | None = None, sc
     *lead, K = x.shape if x.dim() else (0,)
     if K == 0 or K % 32:
         raise ValueError(f"last dim {K} must be a positive multiple of 32")
-    ld, ld_out = _row_stride(x, "x"), 0
+    ld, ld_out, o_ptr = _row_stride(x, "x"), 0, None
+    stream = _launch_stream(x, None if out is True else out, codes, scales)
     if out is True:
-        out, ld_out = x.new_empty(x.shape), K
+        out, ld_out = torch.empty_like(x, memory_format=torch.contiguous_format), K
+        o_ptr = out.data_ptr()
     elif out is not None:
         _need(out, "out", dtype)
         if out.shape != x.shape:
             raise ValueError("out must have x's shape")
-        ld_out = _row_stride(out, "out")
+        ld_out, o_ptr = _row_stride(out, "out"), out.data_ptr()
     if codes is None:
-        codes = x.new_empty((*lead, K // 2), dtype=torch.uint8)
+        codes = torch.empty((*lead, K // 2), dtype=_U8, device=x.device)
     else:
         _mx_field(codes, "codes", (*lead, K // 2))
     if scales is None:
-        scales = x.new_empty((*lead, K // 32), dtype=torch.uint8)
+        scales = torch.empty((*lead, K // 32), dtype=_U8, device=x.device)
     else:
         _mx_field(scales, "scales", (*lead, K // 32))
-    stream = _launch_stream(x, out, codes, scales)
     M = x.numel() // K
     if M:
-        check(lib().dsa_mxfp4_quant(x.data_ptr(), x_type, ld, _ptr(out), ld_out, codes.data_ptr(), scales.data_ptr(),
-                                    M, K, stream), "mxfp4_quant")
+        check(lib().dsa_mxfp4_quant(x.data_ptr(), x_type, ld, o_ptr, ld_out, codes.data_ptr(), scales.data_ptr(), M, K,
+                                    stream), "mxfp4_quant")
     return out, scales, codes
 
 
@@ -407,8 +408,8 @@ def kv_quant_views(cache: torch.Tensor, D: int = 512, rope_dim: int = 64):
         raise ValueError(f"cache must be uint8 with records of {kv_quant_row_bytes(D, rope_dim)} bytes")
     a = D - rope_dim
     b = a + 2 * rope_dim
-    return (cache.narrow(-1, 0, a).view(torch.float8_e4m3fn), cache.narrow(-1, a, b - a).view(BF16),
-            cache.narrow(-1, b, a // 16).view(F32))
+    codes, rope, scales, _ = cache.split((a, b - a, a // 16, cache.shape[-1] - b - a // 16), -1)
+    return codes.view(torch.float8_e4m3fn), rope.view(BF16), scales.view(F32)
 
 
 def _quant_cache(cache: torch.Tensor, B: int, D: int, rope_dim: int) -> None:
@@ -471,14 +472,14 @@ def kv_quant_read(cache: torch.Tensor, idx: torch.Tensor | None = None, D: int =
             raise ValueError(f"idx must be [{B}, K] with a unit stride in the last dim")
         K = idx.shape[1]
         ld = idx.stride(0) if B > 1 else K
+    stream = _launch_stream(cache, idx, out, status)
     if out is None:
-        out = cache.new_empty((B, K, D), dtype=dtype)
+        out = torch.empty((B, K, D), dtype=dtype, device=cache.device)
     else:
         _need(out, "out", dtype)
         _contig(out, "out")
         if out.shape != (B, K, D):
             raise ValueError(f"out must be {(B, K, D)}, got {tuple(out.shape)}")
-    stream = _launch_stream(cache, idx, out, status)
     if B and K:
         check(lib().dsa_kv_quant_read(cache.data_ptr(), cache.stride(0), cache.shape[1], _ptr(idx), ld, out.data_ptr(),
                                       dtype == F32, B, K, D, rope_dim, _ptr(status), stream), "kv_quant_read")
@@ -1020,6 +1021,7 @@ def sparse_attn_quant(q, cache, idx, sink, scale: float, out=None, lse=None, ws:
     if ilead != lead and (S != 1 or ilead not in ([B], [B, 1])):
         raise ValueError(f"idx must be [B, S, K] for q {tuple(q.shape)}, got {tuple(idx.shape)}")
     ld_idx = _row_stride(idx, "idx") if K else 0
+    stream = _launch_stream(q, cache, idx, sink, out, lse, status)
     if out is None:
         out = torch.empty_like(q)
     else:
@@ -1032,14 +1034,13 @@ def sparse_attn_quant(q, cache, idx, sink, scale: float, out=None, lse=None, ws:
         _contig(lse, "lse")
         if lse.numel() != B * S * H:
             raise ValueError(f"lse has {lse.numel()} elements, expected {B * S * H}")
-    stream = _launch_stream(q, cache, idx, sink, out, lse, status)
     if B == 0 or S == 0:
         return out
     L = lib()
     need = L.dsa_sparse_attn_workspace_size(B, S, H, D, K)
     buf = None
     if need:
-        buf = ws.get(need) if ws is not None else q.new_empty(need, dtype=torch.uint8)
+        buf = ws.get(need) if ws is not None else torch.empty(need, dtype=_U8, device=q.device)
     check(L.dsa_sparse_attn_quant(q.data_ptr(), cache.data_ptr(), cache.stride(0), cache.shape[1],
                                   idx.data_ptr() if K else sink.data_ptr(), ld_idx, sink.data_ptr(), out.data_ptr(),
                                   _ptr(lse), B, S, H, D, K, scale, _ptr(buf), need, _ptr(status), stream),
