@@ -468,13 +468,11 @@ __global__ void __launch_bounds__(kQuantThreads) quant_x_kernel(const T* __restr
   for (int64_t w = int64_t(blockIdx.x) * (kQuantThreads / 32) + (threadIdx.x >> 5); w < total; w += step) {
     const int b = int(w / runs), kb0 = int(w - int64_t(b) * runs) * kQuantUnroll;
     const T* src = x + b * ld_x;
-    float v[kQuantUnroll][mx::kVec];
+    mx::Vec8<T> x8[kQuantUnroll];
 #pragma unroll
     for (int u = 0; u < kQuantUnroll; ++u) {
       const int k = (kb0 + u) * KBW + lane * mx::kVec;
-#pragma unroll
-      for (int i = 0; i < mx::kVec; ++i) v[u][i] = 0.f;
-      if (k < K) mx::load8(src + k, v[u]);
+      x8[u] = k < K ? mx::load8(src + k) : mx::zero8<T>();
     }
     const int mt = b / Bt, r = b - mt * Bt;
     const int tile_bytes = Bt * (KBW / 2) + groups * kSfBytes;
@@ -483,14 +481,15 @@ __global__ void __launch_bounds__(kQuantThreads) quant_x_kernel(const T* __restr
     const int at_sf = Bt * (KBW / 2) + (r >> 7) * kSfBytes + (lane >> 4) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4;
 #pragma unroll
     for (int u = 0; u < kQuantUnroll; ++u) {
-      const uint32_t sc = mx::scale_code(v[u]);
+      uint32_t sc;
+      const uint32_t c = mx::quant8<T>(x8[u], sc);
       // blocks 4 j .. 4 j + 3 of the k-block, from lanes 16 j + {0, 4, 8, 12}
       uint32_t word = sc;
       word |= __shfl_down_sync(0xffffffffu, sc, 4) << 8;
       word |= __shfl_down_sync(0xffffffffu, sc, 8) << 16;
       word |= __shfl_down_sync(0xffffffffu, sc, 12) << 24;
       if (kb0 + u < nkb) {
-        *reinterpret_cast<uint32_t*>(tile + u * tile_bytes + at_code) = mx::codes8(v[u], sc);
+        *reinterpret_cast<uint32_t*>(tile + u * tile_bytes + at_code) = c;
         if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(tile + u * tile_bytes + at_sf) = word;
       }
     }

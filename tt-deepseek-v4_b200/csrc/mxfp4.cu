@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(kThreads) mxfp4_quant_kernel(const T* __restri
   const bool flat = ld_x == int64_t(row_chunks) * kVec && (!out || ld_out == ld_x);
   // whole warps stay in the loop: the block maximum is a warp shuffle
   for (int64_t c0 = int64_t(blockIdx.x) * kThreads * kUnroll; c0 < total; c0 += step) {
-    float v[kUnroll][kVec];
+    Vec8<T> x8[kUnroll];
     int64_t at[kUnroll], row[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -52,21 +52,20 @@ __global__ void __launch_bounds__(kThreads) mxfp4_quant_kernel(const T* __restri
         row[u] = at[u] / row_chunks;
         col = (at[u] - row[u] * row_chunks) * kVec;
       }
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) v[u][i] = 0.f;
-      if (at[u] < total) load8(x + row[u] * ld_x + col, v[u]);
+      x8[u] = at[u] < total ? load8(x + row[u] * ld_x + col) : zero8<T>();
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const uint32_t sc = scale_code(v[u]);
+      uint32_t sc;
+      const uint32_t c = quant8<T>(x8[u], sc);
       if (at[u] >= total) continue;
-      const uint32_t c = codes8(v[u], sc);
       codes[at[u]] = c;
       if ((at[u] & 3) == 0) scales[at[u] >> 2] = uint8_t(sc);
       if (out) {
-        values8(c, sc, v[u]);
+        float v[kVec];
+        values8(c, sc, v);
         const int64_t col = flat ? at[u] * kVec : (at[u] - row[u] * row_chunks) * kVec;
-        store8(out + row[u] * ld_out + col, v[u]);
+        store8(out + row[u] * ld_out + col, v);
       }
     }
   }

@@ -23,50 +23,98 @@ namespace mx {
 constexpr int kBlock = 32;
 constexpr int kVec = 8;  // elements a lane holds; a block is 4 neighbouring lanes
 
-// 8 consecutive elements as fp32
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* v) {
-  bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(p)), v);
-}
-__device__ __forceinline__ void load8(const __half* p, float* v) {
-  const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-  const __half2* h = reinterpret_cast<const __half2*>(&w);
+// A lane's 8 consecutive elements as they lie in memory.
+template <typename T>
+struct Vec8 {
+  uint4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Vec8<T> load8(const T* p) {
+  Vec8<T> r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(h[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
+  for (int i = 0; i < int(sizeof(T) / 2); ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  return r;
 }
-__device__ __forceinline__ void load8(const float* p, float* v) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+template <typename T>
+__device__ __forceinline__ Vec8<T> zero8() {
+  Vec8<T> r;
+#pragma unroll
+  for (int i = 0; i < int(sizeof(T) / 2); ++i) r.w[i] = make_uint4(0, 0, 0, 0);
+  return r;
 }
 
-// The scale code of the block whose 32 elements this lane and its three
-// neighbours hold (every lane of the warp calls it).  The fp32 bits without
-// the sign order as integers, NaN and infinity above every number.
-__device__ __forceinline__ uint32_t scale_code(const float* v) {
+__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
+__device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
+// eight fp32 values as E2M1, two a byte, the first in the low half
+__device__ __forceinline__ uint32_t e2m1x8(const float* f) {
+  uint32_t c;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(c)
+      : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+  return c;
+}
+
+// Scale code of the block that this lane and its three neighbours hold (every
+// lane of the warp calls it) and this lane's 8 elements as E2M1 codes.
+// fp32 and fp16: the fp32 bits without the sign order as integers, NaN and
+// infinity above every number.
+template <typename T>
+__device__ __forceinline__ uint32_t quant8(const Vec8<T>& x, uint32_t& sc) {
+  float v[kVec];
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t w[8] = {x.w[0].x, x.w[0].y, x.w[0].z, x.w[0].w, x.w[1].x, x.w[1].y, x.w[1].z, x.w[1].w};
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v[i] = __uint_as_float(w[i]);
+  } else {
+    const __half2* h = reinterpret_cast<const __half2*>(&x.w[0]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(h[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
   const int field = int(m >> 23);
-  return field == 255 ? 255u : uint32_t(max(field - 2, 0));
-}
-
-// this lane's 8 elements as E2M1, two a byte, the even element in the low half
-__device__ __forceinline__ uint32_t codes8(const float* v, uint32_t sc) {
-  if (sc == 255u) return 0u;
+  sc = field == 255 ? 255u : uint32_t(max(field - 2, 0));
   const float inv = __uint_as_float((254u - sc) << 23);
-  uint32_t c = 0;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) v[i] *= inv;
+  return sc == 255u ? 0u : e2m1x8(v);
+}
+// bf16: maximum and scaling two elements an instruction (a power of two, so
+// exact where the code is not zero); the quantisation of a 4096 x 8192
+// activation is bound by instructions, not bytes.
+template <>
+__device__ __forceinline__ uint32_t quant8(const Vec8<__nv_bfloat16>& x, uint32_t& sc) {
+  const uint32_t w[4] = {x.w[0].x, x.w[0].y, x.w[0].z, x.w[0].w};
+  __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(as_bf162(w[0])), __habs2(as_bf162(w[1]))),
+                                 __hmax2_nan(__habs2(as_bf162(w[2])), __habs2(as_bf162(w[3]))));
+  m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  const uint32_t mb = as_u32(m);
+  // the exponent field orders as the number does, NaN and infinity 255
+  const int field = int(max((mb >> 7) & 0xffu, (mb >> 23) & 0xffu));
+  sc = field == 255 ? 255u : uint32_t(max(field - 2, 0));
+  const __nv_bfloat162 inv = as_bf162(((254u - sc) << 7) * 0x10001u);
+  float f[kVec];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __nv_fp4x2_storage_t b =
-        __nv_cvt_float2_to_fp4x2(make_float2(v[2 * i] * inv, v[2 * i + 1] * inv), __NV_E2M1, cudaRoundNearest);
-    c |= uint32_t(b) << (8 * i);
+    const uint32_t y = as_u32(__hmul2(as_bf162(w[i]), inv));
+    f[2 * i] = __uint_as_float(y << 16);
+    f[2 * i + 1] = __uint_as_float(y & 0xffff0000u);
   }
-  return c;
+  return sc == 255u ? 0u : e2m1x8(f);
 }
 
 // the values the codes stand for
