@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
 
 // X [B, K] -> its tiles.  A warp takes kQuantUnroll k-blocks of one token: its
 // lanes hold the 256 elements of a k-block, so it writes the row's 128 B of
-// codes and two words of four scales (past K: zeros).
+// codes and eight scales (past K: zeros).
 constexpr int kQuantThreads = 256;
 constexpr int kQuantUnroll = 4;
 template <typename T>
@@ -466,7 +466,9 @@ __global__ void __launch_bounds__(kQuantThreads) quant_x_kernel(const T* __restr
   const int runs = (nkb + kQuantUnroll - 1) / kQuantUnroll;  // of a token
   const int64_t total = int64_t(B) * runs, step = int64_t(gridDim.x) * (kQuantThreads / 32);
   for (int64_t w = int64_t(blockIdx.x) * (kQuantThreads / 32) + (threadIdx.x >> 5); w < total; w += step) {
-    const int b = int(w / runs), kb0 = int(w - int64_t(b) * runs) * kQuantUnroll;
+    // (a 64-bit division was a quarter of the instructions)
+    const int b = total < (int64_t(1) << 32) ? int(uint32_t(w) / uint32_t(runs)) : int(w / runs);
+    const int kb0 = int(w - int64_t(b) * runs) * kQuantUnroll;
     const T* src = x + b * ld_x;
     mx::Vec8<T> x8[kQuantUnroll];
 #pragma unroll
@@ -474,23 +476,19 @@ __global__ void __launch_bounds__(kQuantThreads) quant_x_kernel(const T* __restr
       const int k = (kb0 + u) * KBW + lane * mx::kVec;
       x8[u] = k < K ? mx::load8(src + k) : mx::zero8<T>();
     }
-    const int mt = b / Bt, r = b - mt * Bt;
+    const int mt = int(uint32_t(b) / uint32_t(Bt)), r = b - mt * Bt;
     const int tile_bytes = Bt * (KBW / 2) + groups * kSfBytes;
     uint8_t* tile = tiles + (int64_t(mt) * nkb + kb0) * tile_bytes;
     const int at_code = r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
-    const int at_sf = Bt * (KBW / 2) + (r >> 7) * kSfBytes + (lane >> 4) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4;
+    const int at_sf = Bt * (KBW / 2) + (r >> 7) * kSfBytes + (lane >> 4) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 +
+                      ((lane >> 2) & 3);
 #pragma unroll
     for (int u = 0; u < kQuantUnroll; ++u) {
       uint32_t sc;
       const uint32_t c = mx::quant8<T>(x8[u], sc);
-      // blocks 4 j .. 4 j + 3 of the k-block, from lanes 16 j + {0, 4, 8, 12}
-      uint32_t word = sc;
-      word |= __shfl_down_sync(0xffffffffu, sc, 4) << 8;
-      word |= __shfl_down_sync(0xffffffffu, sc, 8) << 16;
-      word |= __shfl_down_sync(0xffffffffu, sc, 12) << 24;
       if (kb0 + u < nkb) {
         *reinterpret_cast<uint32_t*>(tile + u * tile_bytes + at_code) = c;
-        if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(tile + u * tile_bytes + at_sf) = word;
+        if ((lane & 3) == 0) tile[u * tile_bytes + at_sf] = uint8_t(sc);
       }
     }
   }
