@@ -239,54 +239,55 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
     __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      const uint32_t id0 = tc::idesc_mxf4(128, a.Bt, 0), id2 = tc::idesc_mxf4(128, a.Bt, 2);
-      const uint32_t hi = tc::desc_hi(1024, tc::kLayoutSw128);
-      const uint32_t sf_step = sf_cols(a.groups), sfb_step = 4 * a.groups;
-      int s = 0, li = 0;
-      uint32_t ph = 0;
-      for (int item = cid; item < n_items; item += n_cl, ++li) {
-        const int acc = li & 1;
-        if (li >= 2) tc::mbar_wait(smem_u32(&aux->acc_empty[acc]), ((li - 2) >> 1) & 1, a.status, 2, a.wait_limit);
+    const uint32_t id0 = tc::idesc_mxf4(128, a.Bt, 0), id2 = tc::idesc_mxf4(128, a.Bt, 2);
+    const uint32_t hi = tc::desc_hi(1024, tc::kLayoutSw128);
+    const uint32_t sf_step = sf_cols(a.groups), sfb_step = 4 * a.groups;
+    int s = 0, li = 0;
+    uint32_t ph = 0;
+    for (int item = cid; item < n_items; item += n_cl, ++li) {
+      const int acc = li & 1;
+      if (li >= 2) tc::mbar_wait(smem_u32(&aux->acc_empty[acc]), ((li - 2) >> 1) & 1, a.status, 2, a.wait_limit);
+      tc::fence_after_sync();
+      const uint32_t d = tmem + uint32_t(kMaxBt) * acc;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const uint32_t st = sbase + s * a.stage_bytes;
+        const uint32_t sfa = tmem + kColSf + sf_step * s, sfb = sfa + 8;
+        const uint32_t a_lo = tc::desc_lo(st, 16), b_lo = tc::desc_lo(st + kWBytes, 16);
+        tc::mbar_wait(smem_u32(&aux->full[s]), ph, a.status, 2, a.wait_limit);
+        tc::mbar_wait(smem_u32(&aux->sf_full[s]), ph, a.status, 2, a.wait_limit);
         tc::fence_after_sync();
-        const uint32_t d = tmem + uint32_t(kMaxBt) * acc;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          const uint32_t st = sbase + s * a.stage_bytes;
-          const uint32_t sfa = tmem + kColSf + sf_step * s, sfb = sfa + 8;
-          const uint32_t a_lo = tc::desc_lo(st, 16), b_lo = tc::desc_lo(st + kWBytes, 16);
-          tc::mbar_wait(smem_u32(&aux->full[s]), ph, a.status, 2, a.wait_limit);
-          tc::mbar_wait(smem_u32(&aux->sf_full[s]), ph, a.status, 2, a.wait_limit);
-          tc::fence_after_sync();
+        if (tc::elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < KBW / 64; ++ks)
             tc::mma_mxf4(d, tc::desc_pack(a_lo + ks * 2, hi), tc::desc_pack(b_lo + ks * 2, hi), (ks & 1) ? id2 : id0,
                          sfa + 4 * (ks >> 1), sfb + sfb_step * (ks >> 1), (kb > kb0 || ks) ? 1u : 0u);
           tc::mma_commit(smem_u32(&aux->empty[s]));
-          if (++s == NS) {
-            s = 0;
-            ph ^= 1;
-          }
         }
-        tc::mma_commit(smem_u32(&aux->acc_full[acc]));
+        __syncwarp();
+        if (++s == NS) {
+          s = 0;
+          ph ^= 1;
+        }
       }
+      if (tc::elect_one()) tc::mma_commit(smem_u32(&aux->acc_full[acc]));
+      __syncwarp();
     }
-    __syncwarp();
   } else if (warp == 6) {
     // ---------------------------------------------------------------- scales
     // A stage's columns are free once its MMAs have completed, which is when
     // the producer refills the stage: the wait for `full` covers both.
-    if (lane == 0) {
-      const uint32_t hi = tc::desc_hi(128, tc::kLayoutNone);
-      const uint32_t sf_step = sf_cols(a.groups);
-      int s = 0;
-      uint32_t ph = 0;
-      for (int item = cid; item < n_items; item += n_cl) {
-        for (int kb = kb0; kb < kb1; ++kb) {
-          const uint32_t st = sbase + s * a.stage_bytes;
-          const uint32_t sfa = tmem + kColSf + sf_step * s;
-          const uint32_t w_lo = tc::desc_lo(st + kCodeBytes, 16), x_lo = tc::desc_lo(st + kWBytes + x_bytes, 16);
-          tc::mbar_wait(smem_u32(&aux->full[s]), ph, a.status, 2, a.wait_limit);
-          tc::fence_after_sync();
+    const uint32_t hi = tc::desc_hi(128, tc::kLayoutNone);
+    const uint32_t sf_step = sf_cols(a.groups);
+    int s = 0;
+    uint32_t ph = 0;
+    for (int item = cid; item < n_items; item += n_cl) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const uint32_t st = sbase + s * a.stage_bytes;
+        const uint32_t sfa = tmem + kColSf + sf_step * s;
+        const uint32_t w_lo = tc::desc_lo(st + kCodeBytes, 16), x_lo = tc::desc_lo(st + kWBytes + x_bytes, 16);
+        tc::mbar_wait(smem_u32(&aux->full[s]), ph, a.status, 2, a.wait_limit);
+        tc::fence_after_sync();
+        if (tc::elect_one()) {
           tc::cp_scales(sfa, tc::desc_pack(w_lo, hi));
           tc::cp_scales(sfa + 4, tc::desc_pack(w_lo + 32, hi));
           if (a.groups == 1) {
@@ -299,14 +300,14 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
             tc::cp_scales(sfa + 20, tc::desc_pack(x_lo + 96, hi));
           }
           tc::mma_commit(smem_u32(&aux->sf_full[s]));
-          if (++s == NS) {
-            s = 0;
-            ph ^= 1;
-          }
+        }
+        __syncwarp();
+        if (++s == NS) {
+          s = 0;
+          ph ^= 1;
         }
       }
     }
-    __syncwarp();
   }
 
   if (warp >= 2 && warp <= 5) {

@@ -32,9 +32,9 @@
 //               128 B at a time only ~4.7 TB/s, so each row is read once,
 //               whole.  A tile completes on its slot's mbarrier through
 //               cp.async.mbarrier.arrive.
-//   warp 8      S issuer (one thread): S(t) as soon as tile t has landed and
+//   warp 8      S issuer: S(t) as soon as tile t has landed and
 //               the softmax has read S(t-1).
-//   warps 4, 12 PV issuers (one thread each, output dims 0-255 / 256-511):
+//   warps 4, 12 PV issuers (output dims 0-255 / 256-511):
 //               PV(t) as soon as P(t) is written (it frees the tile's slot
 //               once both halves completed).  A tcgen05.mma of these shapes
 //               costs ~90 cycles; issuing S and the two PV halves from three
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kQuant ? kQuantThreads : THREADS, 1)
     // kPV0: output dims 0-255 (O^T blocks 0, 1), kPV1: dims 256-511
     if (q_late) q_part();
     const int jb0 = warp == R::kPV0 ? 0 : 2;
-    if (lane == 0 && n > 0) {
+    if (n > 0) {
       const uint32_t hi = tc::desc_hi(1024, tc::kLayoutSw128);
       const uint32_t v_lo = tc::desc_lo(sRing, kPairBytes);  // MN-major: LBO = the next 64 dims (next pair block)
       const uint32_t p_lo = tc::desc_lo(sP, 16);             // K-major rows of 64 keys per head
@@ -548,26 +548,29 @@ __global__ void __launch_bounds__(kQuant ? kQuantThreads : THREADS, 1)
       // PV issuer: PV(np) as soon as P(np) is written (S runs from warp 8)
       for (int np = 0; np < n; ++np) {
         wait(&aux->p_full[np & 1], (np >> 1) & 1);
-        if (*abort_flag) break;
+        if (__any_sync(0xffffffffu, *abort_flag != 0)) break;  // the whole warp
         tc::fence_after_sync();
         const uint32_t vs = v_lo + (np % NT) * (kTileBytes / 16);
         const uint32_t ps = p_lo + (np & 1) * (kPBytes / 16);
+        if (tc::elect_one()) {
 #pragma unroll
-        for (int jb = jb0; jb < jb0 + 2; ++jb) {
+          for (int jb = jb0; jb < jb0 + 2; ++jb) {
 #pragma unroll
-          for (int kk = 0; kk < TK / 16; ++kk) {
-            const uint32_t off = (jb & 1) * 2 * kPairBytes + (jb >> 1) * 2048 + kk * 4096;
-            const uint64_t ad = tc::desc_pack(vs + off / 16, hi);
-            const uint64_t bd = tc::desc_pack(ps + (kk * 32) / 16, hi);
-            tc::mma_bf16(tmem + kColO + H * jb, ad, bd, kIdescPV, (np > 0 || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < TK / 16; ++kk) {
+              const uint32_t off = (jb & 1) * 2 * kPairBytes + (jb >> 1) * 2048 + kk * 4096;
+              const uint64_t ad = tc::desc_pack(vs + off / 16, hi);
+              const uint64_t bd = tc::desc_pack(ps + (kk * 32) / 16, hi);
+              tc::mma_bf16(tmem + kColO + H * jb, ad, bd, kIdescPV, (np > 0 || kk > 0) ? 1u : 0u);
+            }
           }
+          tc::mma_commit(smem_u32(&aux->empty[np % NT]));
+          tc::mma_commit(smem_u32(&aux->pv_done[np & 1]));
         }
-        tc::mma_commit(smem_u32(&aux->empty[np % NT]));
-        tc::mma_commit(smem_u32(&aux->pv_done[np & 1]));
-        if (jb0 == 0) SA_TRACE(kTrPV, np);
+        __syncwarp();
+        if (jb0 == 0 && lane == 0) SA_TRACE(kTrPV, np);
       }
       // every MMA of this CTA has completed before TMEM is released
-      tc::mma_commit(smem_u32(&aux->mma_done));
+      if (tc::elect_one()) tc::mma_commit(smem_u32(&aux->mma_done));
       tc::mbar_wait(smem_u32(&aux->mma_done), 0, a.status, kStatusTimeout, a.wait_limit);
     }
     __syncwarp();
@@ -737,7 +740,7 @@ __global__ void __launch_bounds__(kQuant ? kQuantThreads : THREADS, 1)
   } else if (warp == R::kS) {
     // ------------------------------------------------------------ S issuer
     if (q_late) q_part();
-    if (lane == 0 && n > 0) {
+    if (n > 0) {
       const uint32_t hi = tc::desc_hi(1024, tc::kLayoutSw128);
       const uint32_t k_lo = tc::desc_lo(sRing, 16);  // K-major: LBO unused
       wait(&aux->q_full, 0);
@@ -745,22 +748,25 @@ __global__ void __launch_bounds__(kQuant ? kQuantThreads : THREADS, 1)
       for (int ns = 0; ns < n; ++ns) {
         wait(&aux->full[ns % NT], (ns / NT) & 1);
         if (ns > 0) wait(&aux->s_free, (ns - 1) & 1);
-        if (*abort_flag) break;
+        if (__any_sync(0xffffffffu, *abort_flag != 0)) break;  // the whole warp
         tc::fence_after_sync();
-        SA_TRACE(kTrMmaGot, ns);
+        if (lane == 0) SA_TRACE(kTrMmaGot, ns);
         const uint32_t ks0 = k_lo + (ns % NT) * (kTileBytes / 16);
+        if (tc::elect_one()) {
 #pragma unroll
-        for (int j = 0; j < KB / 2; ++j) {
+          for (int j = 0; j < KB / 2; ++j) {
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const uint64_t bd = tc::desc_pack(ks0 + (j * kPairBytes + ks * 32) / 16, hi);
-            tc::mma_bf16_ts(tmem + kColS, tmem + kColQ + 32 * j + 8 * ks, bd, kIdescS, (j | ks) ? 1u : 0u);
+            for (int ks = 0; ks < 4; ++ks) {
+              const uint64_t bd = tc::desc_pack(ks0 + (j * kPairBytes + ks * 32) / 16, hi);
+              tc::mma_bf16_ts(tmem + kColS, tmem + kColQ + 32 * j + 8 * ks, bd, kIdescS, (j | ks) ? 1u : 0u);
+            }
           }
+          tc::mma_commit(smem_u32(&aux->s_full));
         }
-        tc::mma_commit(smem_u32(&aux->s_full));
-        SA_TRACE(kTrS, ns);
+        __syncwarp();
+        if (lane == 0) SA_TRACE(kTrS, ns);
       }
-      tc::mma_commit(smem_u32(&aux->mma_done));
+      if (tc::elect_one()) tc::mma_commit(smem_u32(&aux->mma_done));
       tc::mbar_wait(smem_u32(&aux->mma_done), 0, a.status, kStatusTimeout, a.wait_limit);
     }
     __syncwarp();
