@@ -98,8 +98,9 @@ int dsa_linear_pack(const void* w, int N, int K, int G, void* packed, size_t pac
  * w_packed: W in the tile layout of dsa_linear_mxfp4_pack (16-byte aligned).
  * K a multiple of 32; B, N, K at most 2^24; x 16-byte aligned, its row stride
  * a multiple of 16 bytes.  workspace: dsa_linear_mxfp4_workspace_size(B, N, K)
- * bytes (the current device's), 16-byte aligned, for X's codes and scales;
- * calls that can overlap need their own.  status (may be NULL): bit 2 when a
+ * bytes (the current device's; 0, and NULL will do, where the product
+ * quantises X itself: a few tokens), 16-byte aligned, for X's codes and
+ * scales; calls that can overlap need their own.  status (may be NULL): bit 2 when a
  * bounded wait ran out.
  * The 4-bit counterpart of dsa_linear; the reference expands such weights
  * (inference.py:283-327). */

@@ -164,8 +164,9 @@ def test_linear_mxfp4_refusals():
     assert L.dsa_linear_mxfp4_packed_bytes(128, 48) == 0 and L.dsa_linear_mxfp4_packed_bytes(0, 64) == 0
     assert L.dsa_linear_mxfp4_packed_bytes(1 << 25, 64) == 0
     assert L.dsa_linear_mxfp4_workspace_size(0, 64, 64) == 0 and L.dsa_linear_mxfp4_workspace_size(4, 64, 48) == 0
-    # one k-block of 32 token rows of codes and the scales of one group of 128 tokens
-    assert L.dsa_linear_mxfp4_workspace_size(4, 64, 64) == 32 * 128 + 1024
+    # a few tokens are quantised by the product itself; many need room for their codes and scales
+    assert L.dsa_linear_mxfp4_workspace_size(4, 64, 64) == 0
+    assert L.dsa_linear_mxfp4_workspace_size(100, 64, 1536) >= 100 * 1536 * 17 // 32
     p = L.dsa_linear_mxfp4_pack
     _refused(p(None, 16, 128, 256, 16, 17408, None), "null")
     _refused(p(16, 16, 128, 250, 16, 17408, None), "multiple of 32")
@@ -188,6 +189,7 @@ def test_linear_mxfp4_refusals():
     _refused(call(x=8), "alignment")
     _refused(call(ld_y=127), "ld_y")
     _refused(call(y=17), "aligned")
-    assert call(wsb=100) == _lib.DSA_ERR_WORKSPACE and "workspace" in _lib.last_error()
-    assert call(ws=None) == _lib.DSA_ERR_WORKSPACE
+    big = dict(B=100, K=1536, ld_x=1536)
+    assert call(wsb=100, **big) == _lib.DSA_ERR_WORKSPACE and "workspace" in _lib.last_error()
+    assert call(ws=None, **big) == _lib.DSA_ERR_WORKSPACE
     assert call(B=0) == _lib.DSA_OK

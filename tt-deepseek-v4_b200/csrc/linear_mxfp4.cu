@@ -6,7 +6,9 @@
 // operand is expanded.
 //
 // Two launches: X's quantisation into tiles of the weight's layout, then the
-// product, whose weight loads start before the first has ended.
+// product, whose weight loads start before the first has ended.  Where a CTA's
+// share of X is a few rows (kFuse), one launch: the epilogue's warps, idle
+// until the first sum, quantise it into shared memory themselves.
 //
 // Weight layout (dsa_linear_mxfp4_pack, once at load time): per (128-row tile
 // t, 256-wide k-block kb) 17 KB: the codes of the 128 rows as a 128-byte
@@ -66,6 +68,7 @@ constexpr int kMaxSplit = 16;
 constexpr int THREADS = 224;
 constexpr int kSmemBytes = 232448;
 constexpr int kAuxBytes = 256;
+constexpr int kFuseUnits = 32;                  // (token, k-block) units of X a CTA quantises itself, at most
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColSf = 2 * kMaxBt;         // scales of each stage: 8 columns of W, 8 a group of X
 __host__ __device__ constexpr int sf_cols(int groups) { return 8 + 8 * groups; }
@@ -77,13 +80,15 @@ static_assert(kWBytes % 1024 == 0, "the swizzled operands start on 1024 B");
 
 struct Args {
   const uint8_t* w;
-  const uint8_t* x;     // X's tiles [m tile][k-block]
+  const uint8_t* x;     // X's tiles [m tile][k-block]; kFuse: X itself
+  int64_t ld_x;         // kFuse: X's row stride, type and columns
+  int x_type, K;
   void* y;
   int64_t ld_y;
   int B, Bt, groups, N, nkb, n_tiles, m_tiles;
   int split, rows_per;  // C CTAs an item; token rows each of them finishes
   int n_stages, tma_store;
-  uint32_t stage_bytes, half_bytes, part_off, recv_off, out_off, aux_off;
+  uint32_t stage_bytes, half_bytes, x_off, part_off, recv_off, out_off, aux_off;
   int32_t* status;
   long long wait_limit;
 };
@@ -95,6 +100,7 @@ struct Aux {
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
   uint64_t ready;
+  uint64_t x_full;
   uint32_t tmem_base;
 };
 static_assert(sizeof(Aux) <= kAuxBytes, "aux block");
@@ -153,7 +159,43 @@ __device__ __forceinline__ void store_rows(const Args& a, int64_t row, int rows,
   }
 }
 
-template <bool kF32>
+// One k-block of one token (a whole warp; elements past K are zero) into a
+// tile of Bt rows: its row of codes and its eight scales.
+template <typename T>
+__device__ __forceinline__ void put_kblock(uint8_t* tile, const mx::Vec8<T>& x, int Bt, int r, int lane) {
+  uint32_t sc;
+  const uint32_t c = mx::quant8<T>(x, sc);
+  *reinterpret_cast<uint32_t*>(tile + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = c;
+  if ((lane & 3) == 0)
+    tile[Bt * (KBW / 2) + (r >> 7) * kSfBytes + (lane >> 4) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 +
+         ((lane >> 2) & 3)] = uint8_t(sc);
+}
+
+// kFuse: the CTA's k-blocks [kb0, kb1) of every token into its tiles at xs
+// (warps w of 4); four (k-block, token) units of a warp in flight
+template <typename T>
+__device__ __forceinline__ void fill_x(const Args& a, uint8_t* xs, uint32_t x_tile, int kb0, int kb1, int w, int lane) {
+  const T* x = reinterpret_cast<const T*>(a.x);
+  const int units = (kb1 - kb0) * a.B;
+  constexpr int kFly = 4;
+  for (int u0 = w; u0 < units; u0 += 4 * kFly) {
+    mx::Vec8<T> v[kFly];
+    int kb[kFly], b[kFly];
+#pragma unroll
+    for (int i = 0; i < kFly; ++i) {
+      const int u = u0 + 4 * i;
+      kb[i] = u / a.B;
+      b[i] = u - kb[i] * a.B;
+      const int k = (kb0 + kb[i]) * KBW + lane * mx::kVec;
+      v[i] = u < units && k < a.K ? mx::load8(x + b[i] * a.ld_x + k) : mx::zero8<T>();
+    }
+#pragma unroll
+    for (int i = 0; i < kFly; ++i)
+      if (u0 + 4 * i < units) put_kblock<T>(xs + kb[i] * x_tile, v[i], a.Bt, b[i], lane);
+  }
+}
+
+template <bool kF32, bool kFuse>
 __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
                                                                   const __grid_constant__ CUtensorMap tm_y) {
   extern __shared__ uint8_t smem_raw[];
@@ -169,7 +211,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
   const int NS = a.n_stages;
   const uint32_t x_bytes = uint32_t(a.Bt) * (KBW / 2);
   const uint32_t x_tile = x_bytes + uint32_t(a.groups) * kSfBytes;
-  const uint32_t stage_tx = kWBytes + x_tile;
+  const uint32_t stage_tx = kFuse ? kWBytes : kWBytes + x_tile;
 
   if (warp == 1) {
     tc::tmem_alloc(smem_u32(&aux->tmem_base), kTmemCols);
@@ -185,6 +227,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
       tc::mbar_init(smem_u32(&aux->acc_full[s]), 1);
       tc::mbar_init(smem_u32(&aux->acc_empty[s]), 4);
     }
+    tc::mbar_init(smem_u32(&aux->x_full), 4);
     tc::mbar_init(smem_u32(&aux->ready), 1);  // the owner's arrival + the copied bytes
     tc::mbar_fence_init();
   }
@@ -228,7 +271,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
             tma::mbar_arrive_expect_tx(fb, stage_tx);
             lin::bulk_load(st, wt, kWBytes, fb);
           }
-          lin::bulk_load(st + kWBytes, xt, x_tile, fb);
+          if constexpr (!kFuse) lin::bulk_load(st + kWBytes, xt, x_tile, fb);
           if (++s == NS) {
             s = 0;
             ph ^= 1;
@@ -244,6 +287,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
     const uint32_t sf_step = sf_cols(a.groups), sfb_step = 4 * a.groups;
     int s = 0, li = 0;
     uint32_t ph = 0;
+    if constexpr (kFuse) tc::mbar_wait(smem_u32(&aux->x_full), 0, a.status, 2, a.wait_limit);
     for (int item = cid; item < n_items; item += n_cl, ++li) {
       const int acc = li & 1;
       if (li >= 2) tc::mbar_wait(smem_u32(&aux->acc_empty[acc]), ((li - 2) >> 1) & 1, a.status, 2, a.wait_limit);
@@ -252,7 +296,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
       for (int kb = kb0; kb < kb1; ++kb) {
         const uint32_t st = sbase + s * a.stage_bytes;
         const uint32_t sfa = tmem + kColSf + sf_step * s, sfb = sfa + 8;
-        const uint32_t a_lo = tc::desc_lo(st, 16), b_lo = tc::desc_lo(st + kWBytes, 16);
+        const uint32_t xt = kFuse ? sbase + a.x_off + (kb - kb0) * x_tile : st + kWBytes;
+        const uint32_t a_lo = tc::desc_lo(st, 16), b_lo = tc::desc_lo(xt, 16);
         tc::mbar_wait(smem_u32(&aux->full[s]), ph, a.status, 2, a.wait_limit);
         tc::mbar_wait(smem_u32(&aux->sf_full[s]), ph, a.status, 2, a.wait_limit);
         tc::fence_after_sync();
@@ -280,11 +325,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
     const uint32_t sf_step = sf_cols(a.groups);
     int s = 0;
     uint32_t ph = 0;
+    if constexpr (kFuse) tc::mbar_wait(smem_u32(&aux->x_full), 0, a.status, 2, a.wait_limit);
     for (int item = cid; item < n_items; item += n_cl) {
       for (int kb = kb0; kb < kb1; ++kb) {
         const uint32_t st = sbase + s * a.stage_bytes;
         const uint32_t sfa = tmem + kColSf + sf_step * s;
-        const uint32_t w_lo = tc::desc_lo(st + kCodeBytes, 16), x_lo = tc::desc_lo(st + kWBytes + x_bytes, 16);
+        const uint32_t xt = kFuse ? sbase + a.x_off + (kb - kb0) * x_tile : st + kWBytes;
+        const uint32_t w_lo = tc::desc_lo(st + kCodeBytes, 16), x_lo = tc::desc_lo(xt + x_bytes, 16);
         tc::mbar_wait(smem_u32(&aux->full[s]), ph, a.status, 2, a.wait_limit);
         tc::fence_after_sync();
         if (tc::elect_one()) {
@@ -318,6 +365,18 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
     uint8_t* stage = smem + a.out_off;
     const bool lead = tid == 64;
     if (lead && a.tma_store) tma::prefetch_map(&tm_y);
+    if constexpr (kFuse) {
+      uint8_t* xs = smem + a.x_off;
+      if (a.x_type == DSA_BF16)
+        fill_x<__nv_bfloat16>(a, xs, x_tile, kb0, kb1, warp - 2, lane);
+      else if (a.x_type == DSA_FP16)
+        fill_x<__half>(a, xs, x_tile, kb0, kb1, warp - 2, lane);
+      else
+        fill_x<float>(a, xs, x_tile, kb0, kb1, warp - 2, lane);
+      tc::fence_proxy_async();  // the tensor cores read it
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(smem_u32(&aux->x_full));
+    }
     if (C == 1) {
       int li = 0;
       for (int item = cid; item < n_items; item += n_cl, ++li) {
@@ -480,18 +539,9 @@ __global__ void __launch_bounds__(kQuantThreads) quant_x_kernel(const T* __restr
     const int mt = int(uint32_t(b) / uint32_t(Bt)), r = b - mt * Bt;
     const int tile_bytes = Bt * (KBW / 2) + groups * kSfBytes;
     uint8_t* tile = tiles + (int64_t(mt) * nkb + kb0) * tile_bytes;
-    const int at_code = r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
-    const int at_sf = Bt * (KBW / 2) + (r >> 7) * kSfBytes + (lane >> 4) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 +
-                      ((lane >> 2) & 3);
 #pragma unroll
-    for (int u = 0; u < kQuantUnroll; ++u) {
-      uint32_t sc;
-      const uint32_t c = mx::quant8<T>(x8[u], sc);
-      if (kb0 + u < nkb) {
-        *reinterpret_cast<uint32_t*>(tile + u * tile_bytes + at_code) = c;
-        if ((lane & 3) == 0) tile[u * tile_bytes + at_sf] = uint8_t(sc);
-      }
-    }
+    for (int u = 0; u < kQuantUnroll; ++u)
+      if (kb0 + u < nkb) put_kblock<T>(tile + u * tile_bytes, x8[u], Bt, r, lane);  // (the warp's: uniform)
   }
 }
 
@@ -540,7 +590,8 @@ static const int* cluster_table() {
   }
   std::call_once(once[dev], [dev] {
     int* n = table[dev];
-    for (auto k : {linear_mxfp4_kernel<false>, linear_mxfp4_kernel<true>}) {
+    for (auto k : {linear_mxfp4_kernel<false, false>, linear_mxfp4_kernel<true, false>, linear_mxfp4_kernel<false, true>,
+                   linear_mxfp4_kernel<true, true>}) {
       if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) != cudaSuccess ||
           cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
         cudaGetLastError();
@@ -560,7 +611,7 @@ static const int* cluster_table() {
       attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
-      if (cudaOccupancyMaxActiveClusters(&n[C], linear_mxfp4_kernel<false>, &cfg) != cudaSuccess) {
+      if (cudaOccupancyMaxActiveClusters(&n[C], linear_mxfp4_kernel<false, false>, &cfg) != cudaSuccess) {
         cudaGetLastError();
         n[C] = 0;
       }
@@ -571,6 +622,7 @@ static const int* cluster_table() {
 
 struct Plan {
   int Bt, m_tiles, groups, split;
+  int fuse;  // k-blocks of X that a CTA quantises itself (0: X is quantised by its own launch)
 };
 
 // shared memory of a plan: the ring's stages (0: it does not fit) and offsets
@@ -579,22 +631,24 @@ static int lay_out(const Plan& p, int B, int es, bool tma_store, Args* a) {
   const int R = (tokens + p.split - 1) / p.split;
   // whole groups of rows as the epilogue writes them: 32, a split's owner 8
   const int out_rows = p.split > 1 ? (R + 7) / 8 * 8 : (p.Bt + 31) / 32 * 32;
-  const uint32_t stage = uint32_t(kWBytes + p.Bt * (KBW / 2) + p.groups * kSfBytes);
+  const uint32_t x_tile = uint32_t(p.Bt * (KBW / 2) + p.groups * kSfBytes);
+  const uint32_t stage = kWBytes + (p.fuse ? 0u : x_tile), x_region = uint32_t(p.fuse) * x_tile;
   const uint32_t out_bytes = tma_store ? (uint32_t(out_rows) * TILE_N * es + 1023u) & ~1023u : 0u;
   const uint32_t part = p.split > 1 ? uint32_t((tokens + 31) / 32 * 32) * TILE_N * 4 : 0u;
   const uint32_t recv = p.split > 1 ? uint32_t(p.split * R) * TILE_N * 4 : 0u;
   const uint32_t room = kSmemBytes - 1024 - kAuxBytes;
-  if (out_bytes >= room || part + recv + out_bytes > room) return 0;
-  const int stages = std::min<int>(max_stages(p.groups), (room - out_bytes) / stage);
+  if (out_bytes + x_region >= room || part + recv + out_bytes > room) return 0;
+  const int stages = std::min<int>(max_stages(p.groups), (room - out_bytes - x_region) / stage);
   if (stages < 2) return 0;
   // the partials take the ring's place; the staged tile starts on 1024 B
-  const uint32_t ring = (std::max(stages * stage, part + recv) + 1023u) & ~1023u;
+  const uint32_t ring = (std::max(stages * stage + x_region, part + recv) + 1023u) & ~1023u;
   if (ring + out_bytes > room) return 0;
   if (a) {
     a->n_stages = stages;
     a->stage_bytes = stage;
     a->rows_per = R;
     a->half_bytes = uint32_t(out_rows) * 128;
+    a->x_off = stages * stage;
     a->part_off = 0;
     a->recv_off = part;
     a->out_off = ring;
@@ -621,7 +675,7 @@ static Plan pick_plan(int B, int N, int nkb) {
   static thread_local Asked last{};
   if (last.clusters == clusters && last.B == B && last.N == N && last.nkb == nkb) return last.plan;
   const int n_tiles = (N + TILE_N - 1) / TILE_N;
-  Plan best{0, 0, 0, 0};
+  Plan best{};
   double best_cost = 0;
   for (int want : {32, 48, 64, 96, 128, 160, 192}) {
     const int m_tiles = (B + want - 1) / want;
@@ -630,7 +684,7 @@ static Plan pick_plan(int B, int N, int nkb) {
     const double kb_cost = std::max((kWBytes + Bt * 136.0) / 48.0, std::max(360.0, 2.0 * Bt));
     for (int C = 1; C <= std::min(kMaxSplit, nkb); ++C) {
       if (C > 1 && items > clusters[C]) continue;
-      Plan p{Bt, m_tiles, (Bt + 127) / 128, C};
+      Plan p{Bt, m_tiles, (Bt + 127) / 128, C, 0};
       if (!lay_out(p, B, 4, true, nullptr)) continue;
       const int64_t waves = C > 1 ? 1 : (items + clusters[1] - 1) / clusters[1];
       const double cost = waves * ((nkb + C - 1) / C * kb_cost + 1500) + Bt * 8.0 + 2000 + (C > 1 ? 3000 + Bt * 16.0 : 0);
@@ -640,11 +694,24 @@ static Plan pick_plan(int B, int N, int nkb) {
       }
     }
   }
+  // Quantising X in the product saves a launch and X's way through memory and
+  // costs each CTA its share of X on four warps.  Measured, fused against two
+  // launches: 1 x 1024 x 4096 (2 units a CTA) 4.85 / 5.81 us, 8 x 1024 x 4096
+  // (16) 5.71 / 6.46, 12 x 1024 x 4096 (24) 6.45 / 6.39, 8 x 32768 x 1024 (32)
+  // 6.82 / 6.82, 16 x 1024 x 4096 (32) 6.87 / 6.52, 24 x 1024 x 4096 (48) 7.87 /
+  // 6.66; a launch is ~5 us of the host's time.
+  const int share = (nkb + best.split - 1) / best.split;
+  if (best.m_tiles == 1 && int64_t(share) * B <= kFuseUnits) {
+    Plan f = best;
+    f.fuse = share;
+    if (lay_out(f, B, 4, true, nullptr)) best = f;
+  }
   last = {clusters, B, N, nkb, best};
   return best;
 }
 
 static size_t x_bytes_for(const Plan& p, int nkb) {
+  if (p.fuse) return 0;
   return size_t(p.m_tiles) * nkb * (p.Bt * (KBW / 2) + p.groups * kSfBytes);
 }
 static int n_kblocks(int K) { return (K + KBW - 1) / KBW; }
@@ -701,7 +768,7 @@ extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const v
   const int nkb = lmx::n_kblocks(K);
   const lmx::Plan p = lmx::pick_plan(B, N, nkb);
   const size_t need = lmx::x_bytes_for(p, nkb);
-  if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)) {
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16))) {
     set_error("linear_mxfp4: needs %zu bytes of 16-byte aligned workspace (got %zu)", need, workspace_bytes);
     return DSA_ERR_WORKSPACE;
   }
@@ -710,7 +777,10 @@ extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const v
 
   lmx::Args a{};
   a.w = static_cast<const uint8_t*>(w_packed);
-  a.x = tiles;
+  a.x = p.fuse ? static_cast<const uint8_t*>(x) : tiles;
+  a.ld_x = ld_x;
+  a.x_type = x_type;
+  a.K = K;
   a.y = y;
   a.ld_y = ld_y;
   a.B = B;
@@ -747,21 +817,23 @@ extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const v
       return DSA_ERR_CUDA;
     }
   }
-  const int64_t q_warps = int64_t(B) * ((nkb + lmx::kQuantUnroll - 1) / lmx::kQuantUnroll);
-  const int per = lmx::kQuantThreads / 32;
-  const dim3 qgrid(unsigned(std::min<int64_t>((q_warps + per - 1) / per, int64_t(num_sms()) * 32)));
-  auto quant = [&](auto* ptr) {
-    using T = std::remove_pointer_t<decltype(ptr)>;
-    launch_pdl(lmx::quant_x_kernel<T>, qgrid, dim3(lmx::kQuantThreads), 0, st, static_cast<const T*>(x), ld_x,
-               tiles, B, K, p.Bt, p.groups, nkb);
-  };
-  if (x_type == DSA_BF16)
-    quant(static_cast<__nv_bfloat16*>(nullptr));
-  else if (x_type == DSA_FP16)
-    quant(static_cast<__half*>(nullptr));
-  else
-    quant(static_cast<float*>(nullptr));
-  DSA_CHECK_LAUNCH("linear_mxfp4 (quantisation)");
+  if (!p.fuse) {
+    const int64_t q_warps = int64_t(B) * ((nkb + lmx::kQuantUnroll - 1) / lmx::kQuantUnroll);
+    const int per = lmx::kQuantThreads / 32;
+    const dim3 qgrid(unsigned(std::min<int64_t>((q_warps + per - 1) / per, int64_t(num_sms()) * 32)));
+    auto quant = [&](auto* ptr) {
+      using T = std::remove_pointer_t<decltype(ptr)>;
+      launch_pdl(lmx::quant_x_kernel<T>, qgrid, dim3(lmx::kQuantThreads), 0, st, static_cast<const T*>(x), ld_x,
+                 tiles, B, K, p.Bt, p.groups, nkb);
+    };
+    if (x_type == DSA_BF16)
+      quant(static_cast<__nv_bfloat16*>(nullptr));
+    else if (x_type == DSA_FP16)
+      quant(static_cast<__half*>(nullptr));
+    else
+      quant(static_cast<float*>(nullptr));
+    DSA_CHECK_LAUNCH("linear_mxfp4 (quantisation)");
+  }
   const int64_t items = int64_t(a.n_tiles) * a.m_tiles;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(p.split > 1 ? items * p.split : std::min<int64_t>(items, num_sms())));
@@ -777,7 +849,9 @@ extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const v
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.split > 1 ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, out_f32 ? lmx::linear_mxfp4_kernel<true> : lmx::linear_mxfp4_kernel<false>, a, tm_y);
+  auto kernel = p.fuse ? (out_f32 ? lmx::linear_mxfp4_kernel<true, true> : lmx::linear_mxfp4_kernel<false, true>)
+                       : (out_f32 ? lmx::linear_mxfp4_kernel<true, false> : lmx::linear_mxfp4_kernel<false, false>);
+  cudaLaunchKernelEx(&cfg, kernel, a, tm_y);
   DSA_CHECK_LAUNCH("linear_mxfp4");
   return DSA_OK;
 }

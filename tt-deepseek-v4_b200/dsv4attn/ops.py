@@ -245,7 +245,8 @@ def linear_mxfp4(x: torch.Tensor, w: MXFP4Weight, out: torch.Tensor | None = Non
     (dsa_linear_mxfp4): x [B, K] bf16, fp16 or fp32 (row stride a multiple of
     16 bytes), quantised to MXFP4 in the call, ``w`` an MXFP4Weight -> y [B, N]
     bf16, or the fp32 sums with ``out_f32``.  Without ``ws`` the scratch (x's
-    codes and scales) is allocated on the current stream for this call."""
+    codes and scales, where the product does not quantise x itself) is
+    allocated on the current stream for this call."""
     _need(x, "x")
     x_type = _X_TYPES.get(x.dtype)
     if x_type is None:
@@ -268,9 +269,11 @@ def linear_mxfp4(x: torch.Tensor, w: MXFP4Weight, out: torch.Tensor | None = Non
         return out
     L = lib()
     need = L.dsa_linear_mxfp4_workspace_size(B, N, K)
-    buf = ws.get(need) if ws is not None else torch.empty(need, dtype=_U8, device=x.device)
+    buf = None
+    if need:
+        buf = ws.get(need) if ws is not None else torch.empty(need, dtype=_U8, device=x.device)
     check(L.dsa_linear_mxfp4(x.data_ptr(), x_type, x.stride(0), w.packed.data_ptr(), out.data_ptr(), out.stride(0),
-                             B, N, K, out_f32, buf.data_ptr(), need, _ptr(status), stream), "linear_mxfp4")
+                             B, N, K, out_f32, _ptr(buf), need, _ptr(status), stream), "linear_mxfp4")
     return out
 
 
