@@ -80,6 +80,23 @@ def weight_bf16(w) -> torch.Tensor:
     raise ValueError(f"unsupported weight dtype {t.dtype} for the attention projections")
 
 
+def mxfp4_parts(w):
+    """``(codes [out, in/2], scales [out, in/32])`` of an MXFP4 Linear weight -
+    a float4_e2m1fn_x2 or int8 tensor of two E2M1 elements a byte that carries
+    one float8_e8m0fnu (or uint8) ``scale`` for each 32 inputs, on the tensor
+    or on its module (inference.py:283-327) - or None for any other weight."""
+    t = getattr(w, "weight", w)
+    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.dtype not in (torch.float4_e2m1fn_x2, torch.int8):
+        return None
+    scale = getattr(t, "scale", None)
+    if scale is None:
+        scale = getattr(w, "scale", None)
+    if not isinstance(scale, torch.Tensor) or scale.dtype not in (torch.float8_e8m0fnu, torch.uint8) \
+            or 32 * scale.shape[-1] != 2 * t.shape[1]:
+        return None
+    return t.detach().view(torch.uint8), scale.detach().view(torch.uint8)
+
+
 def _gamma_of(norm, fallback=None) -> torch.Tensor:
     for name in ("_cpu_gamma", "gamma", "weight"):
         g = getattr(norm, name, None) if norm is not None else None
@@ -113,10 +130,21 @@ class DeviceLinear:
 
     ``fused(device, [w_a, w_b])`` concatenates weights along the output dim
     and records ``_fused_*_out`` widths like the reference's fused
-    DeviceColLinear (inference.py:4954-4966, 5941-5953)."""
+    DeviceColLinear (inference.py:4954-4966, 5941-5953).
+
+    An MXFP4 weight (mxfp4_parts) stays at 4 bits: the product is
+    ``ops.linear_mxfp4``, which quantises x to MXFP4 too and rounds its fp32
+    sums once (``out_dtype=F32``: not at all); ``scale`` must then be 1."""
 
     def __init__(self, device, weight, scale: float = 1.0, out_dtype=BF16):
         self.device = _device_of(device)
+        parts = mxfp4_parts(weight)
+        if parts is not None:
+            if scale != 1.0:
+                raise ValueError("an MXFP4 weight takes no scale")
+            self._set_mxfp4(*parts)
+            self.out_dtype = out_dtype
+            return
         w = weight_bf16(weight)
         if scale != 1.0:
             w = (w.float() * scale).to(BF16)
@@ -125,8 +153,21 @@ class DeviceLinear:
         self.weight = ops.pack_linear_weight(w.to(self.device).contiguous())
         self.out_dtype = out_dtype
 
+    def _set_mxfp4(self, codes, scales):
+        self.out_dim, self.in_dim = codes.shape[0], 2 * codes.shape[1]
+        self.weight = ops.pack_linear_weight_mxfp4(codes.to(self.device).contiguous(),
+                                                   scales.to(self.device).contiguous())
+
     @classmethod
     def fused(cls, device, weights, names=("kv", "gate")):
+        parts = [mxfp4_parts(w) for w in weights]
+        if all(p is not None for p in parts):
+            lin = cls.__new__(cls)
+            lin.device, lin.out_dtype = _device_of(device), BF16
+            lin._set_mxfp4(torch.cat([c for c, _ in parts], 0), torch.cat([s for _, s in parts], 0))
+            for n, (c, _) in zip(names, parts):
+                setattr(lin, f"_fused_{n}_out", c.shape[0])
+            return lin
         ws = [weight_bf16(w) for w in weights]
         lin = cls(device, torch.cat(ws, 0))
         for n, w in zip(names, ws):
@@ -141,6 +182,15 @@ class DeviceLinear:
             raise ValueError(f"input dim {x.shape[-1]} != weight in_dim {self.in_dim}")
         lead = x.shape[:-1]
         x2 = x.reshape(-1, self.in_dim).to(BF16).contiguous()
+        if isinstance(self.weight, ops.MXFP4Weight):
+            y = ops.linear_mxfp4(x2, self.weight, out_f32=self.out_dtype != BF16, status=status)
+            if rope is not None:
+                cos, sin, pos, head_dim, rope_dim = rope[:5]
+                if len(rope) > 5 and rope[5] or self.out_dtype != BF16 or self.out_dim % head_dim:
+                    raise ValueError("the rotary of an MXFP4 projection covers every head of a bf16 result")
+                ops.head_norm_rope(y, self.out_dim // head_dim, head_dim, cos, sin, pos, rope_dim, norm=False, out=y,
+                                   status=status)
+            return y.reshape(*lead, self.out_dim)
         y = ops.linear(x2, self.weight, out_f32=self.out_dtype != BF16, rope=rope, status=status)
         return y.reshape(*lead, self.out_dim)
 
@@ -206,7 +256,8 @@ class DeviceSparseAttn(torch.nn.Module):
 
     def forward_device(self, q_tt, kv_tt, idxs_tt, valid_tt, S: int, K: int, out=None):
         """q_tt [B, S, H, D] bf16 (pre-scaled); kv_tt [N, D] (B == 1) or
-        [B, N, D]; idxs_tt [B, S*K] int32; valid_tt None (sentinels in the
+        [B, N, D] bf16, or the FP8 latent cache [B, N, 608] uint8
+        (ops.kv_quant_cache); idxs_tt [B, S*K] int32; valid_tt None (sentinels in the
         indices) or the reference's additive bf16 {0, -inf} mask [B, S, 1, K]
         over clamped indices.  Returns o [B, S, H, D] bf16."""
         B, Sq, H, D = q_tt.shape
@@ -219,6 +270,8 @@ class DeviceSparseAttn(torch.nn.Module):
         idx = idxs_tt.reshape(B, S, K)
         if valid_tt is not None:
             idx = ops.fold_index_mask(idx.contiguous(), valid_tt.reshape(B, S, K).contiguous())
+        if kv_tt.dtype == torch.uint8:
+            return ops.sparse_attn_quant(q_tt, kv_tt, idx, self.sink, 1.0, out=out, ws=self.ws, status=self.status)
         if kv_tt.dim() == 2 and B != 1:
             raise ValueError("a flat [N, D] kv needs B == 1; pass [B, N, D]")
         return ops.sparse_attn(q_tt, kv_tt, idx, self.sink, 1.0, out=out, ws=self.ws, status=self.status)
