@@ -158,6 +158,18 @@ def test_non_finite_blocks_read_nan(cuda_dev):
     assert torch.equal(got[0][~nan], want[0][~nan])
 
 
+def test_more_sequences_than_a_grid_dimension(cuda_dev):
+    from dsv4attn import ops
+    B = 66_000
+    kv = _kv(B, 1, 128, seed=2).to(cuda_dev)
+    cache = ops.kv_quant_cache(B, 2, 128, 0, device=cuda_dev)
+    pos = (torch.arange(B, dtype=I32) % 5).to(cuda_dev)
+    ops.kv_quant_write(kv, cache, pos, 2, rope_dim=0)
+    got = ops.kv_quant_read(cache, (pos % 2).view(B, 1), D=128, rope_dim=0)
+    other = ops.kv_quant_read(cache, (1 - pos % 2).view(B, 1), D=128, rope_dim=0)
+    assert torch.equal(_bits(got).cpu(), _bits(_want_rows(kv.cpu(), 0)[2])) and bool((other == 0).all())
+
+
 def test_write_strided_kv_and_a_wider_cache(cuda_dev):
     """kv as a column slice of a wider projection output, batch and token
     strides swapped; a cache of more sequences than the call writes."""

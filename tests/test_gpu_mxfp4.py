@@ -123,7 +123,8 @@ def _check_linear(y, x, codes, scales):
 
 SIZES = [(1, 1, 32), (1, 128, 256), (2, 7, 64), (1, 1024, 4096), (31, 200, 96), (32, 129, 288), (33, 64, 4096),
          (64, 2048, 1024), (64, 512, 4096), (100, 2001, 512), (128, 256, 8192), (192, 384, 256), (193, 130, 544),
-         (333, 2001, 4128), (400, 64, 32), (1000, 300, 2080), (2, 24000, 1024), (700, 8200, 512), (5, 1, 8192)]
+         (333, 2001, 4128), (400, 64, 32), (1000, 300, 2080), (2, 24000, 1024), (700, 8200, 512), (5, 1, 8192),
+         (3, 8, 64), (40, 16, 512), (200, 40, 320), (65, 72, 2048), (17, 136, 8192), (1, 32768, 1024)]
 
 
 @pytest.mark.parametrize("B,N,K", SIZES)

@@ -236,8 +236,11 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
   tc::fence_after_sync();
   const uint32_t tmem = aux->tmem_base;
 
-  // the weights come from no kernel of this call: their first tiles are
-  // requested before the dependency wait, X's codes and scales after it
+  // The weights' first tiles are requested before the dependency wait: the
+  // kernel before this one is x's quantisation, which let it start only after
+  // its own wait, so whatever wrote the weights has completed.  kFuse: the
+  // kernel before may be the one that packed them.
+  if constexpr (kFuse) pdl_wait();
   int npre = 0;
   if (warp == 0 && lane == 0) {
     for (int item = cid; item < n_items && npre < NS; item += n_cl) {
@@ -249,7 +252,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
       }
     }
   }
-  pdl_wait();
+  if constexpr (!kFuse) pdl_wait();
   pdl_launch_dependents();
 
   // a stage's address, barrier and parity advance by counters: a division a
@@ -696,10 +699,10 @@ static Plan pick_plan(int B, int N, int nkb) {
   }
   // Quantising X in the product saves a launch and X's way through memory and
   // costs each CTA its share of X on four warps.  Measured, fused against two
-  // launches: 1 x 1024 x 4096 (2 units a CTA) 4.85 / 5.81 us, 8 x 1024 x 4096
-  // (16) 5.71 / 6.46, 12 x 1024 x 4096 (24) 6.45 / 6.39, 8 x 32768 x 1024 (32)
-  // 6.82 / 6.82, 16 x 1024 x 4096 (32) 6.87 / 6.52, 24 x 1024 x 4096 (48) 7.87 /
-  // 6.66; a launch is ~5 us of the host's time.
+  // launches: 1 x 1024 x 4096 (2 units a CTA) 4.8 / 5.8 us, 8 x 1024 x 4096
+  // (16) 5.8 / 6.5, 12 x 1024 x 4096 (24) 6.4 / 6.4, 8 x 32768 x 1024 (32) 6.9 /
+  // 6.8, 16 x 1024 x 4096 (32) 6.9 / 6.5, 24 x 1024 x 4096 (48) 7.9 / 6.7; a
+  // launch more is ~5 us of the host's time, hence 32.
   const int share = (nkb + best.split - 1) / best.split;
   if (best.m_tiles == 1 && int64_t(share) * B <= kFuseUnits) {
     Plan f = best;
@@ -767,6 +770,7 @@ extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const v
   if (B == 0) return DSA_OK;
   const int nkb = lmx::n_kblocks(K);
   const lmx::Plan p = lmx::pick_plan(B, N, nkb);
+  DSA_CHECK_ARG(int64_t((N + lmx::TILE_N - 1) / lmx::TILE_N) * p.m_tiles <= INT32_MAX, "linear_mxfp4: B*N is too large");
   const size_t need = lmx::x_bytes_for(p, nkb);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16))) {
     set_error("linear_mxfp4: needs %zu bytes of 16-byte aligned workspace (got %zu)", need, workspace_bytes);
