@@ -661,10 +661,14 @@ static int lay_out(const Plan& p, int B, int es, bool tma_store, Args* a) {
 }
 
 // Tokens an item and CTAs an item: the pair with the lowest estimate of the
-// busiest CTA's cycles.  A k-block costs what its bytes take to reach the SM
-// (~48 B a cycle) and at least its four MMAs (~90 cycles each, 2 Bt at full
-// rate); an item costs a fixed ~2K cycles and its share of the epilogue, a
-// split ~3K more and the exchange of its partials.
+// busiest CTA's cycles.  A k-block takes its issuers ~550 cycles and its bytes
+// ~70 a cycle into the SM (at 192 tokens 630 measured); an item a fixed ~1.5K
+// cycles and its share of the epilogue; a split its cluster's start and
+// barriers, the exchange of its partial and the sum of C of them.  Half of the
+// time that all bytes would take at 50 a cycle and SM breaks ties towards
+// fewer re-reads.  Measured over 18 shapes x 60 pairs the pick is within 7 % of the
+// best; splitting pays below ~64 tokens (64 x 4096 x 8192: 11.1 us with C = 4,
+// 128 x 4096 x 8192: 15.4 with C = 4, 13.4 unsplit).
 static Plan pick_plan(int B, int N, int nkb) {
   static const int kNone[kMaxSplit + 1] = {0, 148};  // no device: unsplit
   const int* clusters = cluster_table();
@@ -684,13 +688,16 @@ static Plan pick_plan(int B, int N, int nkb) {
     const int m_tiles = (B + want - 1) / want;
     const int Bt = std::max(32, ((B + m_tiles - 1) / m_tiles + 15) / 16 * 16);
     const int64_t items = int64_t(n_tiles) * m_tiles;
-    const double kb_cost = std::max((kWBytes + Bt * 136.0) / 48.0, std::max(360.0, 2.0 * Bt));
+    const double tokens = std::min(B, Bt);
+    const double kb_bytes = kWBytes + Bt * 136.0, kb_cost = std::max(550.0, kb_bytes / 70.0);
+    const double all_bytes = items * double(nkb) * kb_bytes / (50.0 * clusters[1]);
     for (int C = 1; C <= std::min(kMaxSplit, nkb); ++C) {
       if (C > 1 && items > clusters[C]) continue;
       Plan p{Bt, m_tiles, (Bt + 127) / 128, C, 0};
       if (!lay_out(p, B, 4, true, nullptr)) continue;
       const int64_t waves = C > 1 ? 1 : (items + clusters[1] - 1) / clusters[1];
-      const double cost = waves * ((nkb + C - 1) / C * kb_cost + 1500) + Bt * 8.0 + 2000 + (C > 1 ? 3000 + Bt * 16.0 : 0);
+      const double cost = waves * ((nkb + C - 1) / C * kb_cost + 1500) + Bt * 8.0 + 0.5 * all_bytes +
+                          (C > 1 ? 3000 + (40.0 + 0.4 * tokens) * tokens + 250.0 * C : 0);
       if (best.Bt == 0 || cost < best_cost) {
         best_cost = cost;
         best = p;
@@ -770,6 +777,10 @@ extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const v
   if (B == 0) return DSA_OK;
   const int nkb = lmx::n_kblocks(K);
   const lmx::Plan p = lmx::pick_plan(B, N, nkb);
+  if (p.Bt == 0) {
+    set_error("linear_mxfp4: no launch configuration fits");
+    return DSA_ERR_CUDA;
+  }
   DSA_CHECK_ARG(int64_t((N + lmx::TILE_N - 1) / lmx::TILE_N) * p.m_tiles <= INT32_MAX, "linear_mxfp4: B*N is too large");
   const size_t need = lmx::x_bytes_for(p, nkb);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16))) {
