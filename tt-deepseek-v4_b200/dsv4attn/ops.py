@@ -267,13 +267,13 @@ def linear_mxfp4(x: torch.Tensor, w: MXFP4Weight, out: torch.Tensor | None = Non
             raise ValueError(f"out must be [{B}, >={N}] with contiguous rows, got {tuple(out.shape)}")
     if B == 0:
         return out
-    L = lib()
-    need = L.dsa_linear_mxfp4_workspace_size(B, N, K)
+    need = _linear_ws[x.get_device(), B, N, K]
     buf = None
     if need:
         buf = ws.get(need) if ws is not None else torch.empty(need, dtype=_U8, device=x.device)
-    check(L.dsa_linear_mxfp4(x.data_ptr(), x_type, x.stride(0), w.packed.data_ptr(), out.data_ptr(), out.stride(0),
-                             B, N, K, out_f32, _ptr(buf), need, _ptr(status), stream), "linear_mxfp4")
+    check(lib().dsa_linear_mxfp4(x.data_ptr(), x_type, x.stride(0), w.packed.data_ptr(), out.data_ptr(),
+                                 out.stride(0), B, N, K, out_f32, None if buf is None else buf.data_ptr(), need,
+                                 None if status is None else status.data_ptr(), stream), "linear_mxfp4")
     return out
 
 
@@ -305,6 +305,24 @@ def act_quant_block(x: torch.Tensor, block: int = 64, fp8_max: float = 448.0, ep
           "act_quant_block")
     return out, scales, codes
 
+
+class _Sizes(dict):
+    """Workspace sizes already asked for, by shape and device: host arithmetic
+    of the library that a call would repeat (0.1 against 0.8 us)."""
+
+    def __init__(self, ask):
+        super().__init__()
+        self.ask = ask
+
+    def __missing__(self, key):
+        if len(self) >= 4096:
+            self.clear()
+        n = self[key] = int(self.ask(*key[1:]))
+        return n
+
+
+_linear_ws = _Sizes(lambda B, N, K: lib().dsa_linear_mxfp4_workspace_size(B, N, K))
+_attn_ws = _Sizes(lambda B, S, K: lib().dsa_sparse_attn_workspace_size(B, S, 64, 512, K))
 
 _X_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _U8 = torch.uint8
@@ -355,27 +373,27 @@ def mxfp4_quant(x: torch.Tensor, out=None, codes: torch.Tensor | None = None, sc
     x_type = _X_TYPES.get(dtype)
     if x_type is None:
         raise ValueError(f"x must be bfloat16, float16 or float32, got {dtype}")
-    *lead, K = x.shape if x.dim() else (0,)
+    lead, K = x.shape[:-1], x.shape[-1] if x.dim() else 0
     if K == 0 or K % 32:
         raise ValueError(f"last dim {K} must be a positive multiple of 32")
     ld, ld_out, o_ptr = _row_stride(x, "x"), 0, None
     stream = _launch_stream(x, None if out is True else out, codes, scales)
     if out is True:
-        out, ld_out = torch.empty_like(x, memory_format=torch.contiguous_format), K
-        o_ptr = out.data_ptr()
+        out = torch.empty_like(x) if ld == K else x.new_empty(x.shape)
+        ld_out, o_ptr = K, out.data_ptr()
     elif out is not None:
         _need(out, "out", dtype)
         if out.shape != x.shape:
             raise ValueError("out must have x's shape")
         ld_out, o_ptr = _row_stride(out, "out"), out.data_ptr()
     if codes is None:
-        codes = torch.empty((*lead, K // 2), dtype=_U8, device=x.device)
+        codes = torch.empty(lead + (K // 2,), dtype=_U8, device=x.device)
     else:
-        _mx_field(codes, "codes", (*lead, K // 2))
+        _mx_field(codes, "codes", lead + (K // 2,))
     if scales is None:
-        scales = torch.empty((*lead, K // 32), dtype=_U8, device=x.device)
+        scales = torch.empty(lead + (K // 32,), dtype=_U8, device=x.device)
     else:
-        _mx_field(scales, "scales", (*lead, K // 32))
+        _mx_field(scales, "scales", lead + (K // 32,))
     M = x.numel() // K
     if M:
         check(lib().dsa_mxfp4_quant(x.data_ptr(), x_type, ld, o_ptr, ld_out, codes.data_ptr(), scales.data_ptr(), M, K,
@@ -416,13 +434,15 @@ def kv_quant_views(cache: torch.Tensor, D: int = 512, rope_dim: int = 64):
 
 
 def _quant_cache(cache: torch.Tensor, B: int, D: int, rope_dim: int) -> None:
-    _need(cache, "cache", torch.uint8)
+    _need(cache, "cache", _U8)
     rb = kv_quant_row_bytes(D, rope_dim)
-    shape = cache.shape
-    if len(shape) != 3 or shape[0] < B or shape[2] != rb or shape[1] < 1 \
-            or cache.stride()[1:] != (rb, 1) and (cache.stride(2) != 1 or shape[1] > 1):
-        raise ValueError(f"cache must be [>={B}, rows, {rb}] with contiguous rows (D={D}, rope_dim={rope_dim}), "
-                         f"got {tuple(cache.shape)}")
+    if cache.dim() == 3:
+        n, rows, width = cache.shape
+        _, row, one = cache.stride()
+        if n >= B and rows >= 1 and width == rb and one == 1 and (row == rb or rows == 1):
+            return
+    raise ValueError(f"cache must be [>={B}, rows, {rb}] with contiguous rows (D={D}, rope_dim={rope_dim}), "
+                     f"got {tuple(cache.shape)}")
 
 
 def _per_sequence(t, name: str, B: int) -> None:
@@ -1039,15 +1059,15 @@ def sparse_attn_quant(q, cache, idx, sink, scale: float, out=None, lse=None, ws:
             raise ValueError(f"lse has {lse.numel()} elements, expected {B * S * H}")
     if B == 0 or S == 0:
         return out
-    L = lib()
-    need = L.dsa_sparse_attn_workspace_size(B, S, H, D, K)
+    need = _attn_ws[q.get_device(), B, S, K]
     buf = None
     if need:
         buf = ws.get(need) if ws is not None else torch.empty(need, dtype=_U8, device=q.device)
-    check(L.dsa_sparse_attn_quant(q.data_ptr(), cache.data_ptr(), cache.stride(0), cache.shape[1],
-                                  idx.data_ptr() if K else sink.data_ptr(), ld_idx, sink.data_ptr(), out.data_ptr(),
-                                  _ptr(lse), B, S, H, D, K, scale, _ptr(buf), need, _ptr(status), stream),
-          "sparse_attn_quant")
+    check(lib().dsa_sparse_attn_quant(q.data_ptr(), cache.data_ptr(), cache.stride(0), cache.shape[1],
+                                      idx.data_ptr() if K else sink.data_ptr(), ld_idx, sink.data_ptr(),
+                                      out.data_ptr(), None if lse is None else lse.data_ptr(), B, S, H, D, K, scale,
+                                      None if buf is None else buf.data_ptr(), need,
+                                      None if status is None else status.data_ptr(), stream), "sparse_attn_quant")
     return out
 
 
