@@ -159,39 +159,56 @@ __device__ __forceinline__ void store_rows(const Args& a, int64_t row, int rows,
   }
 }
 
-// One k-block of one token (a whole warp; elements past K are zero) into a
-// tile of Bt rows: its row of codes and its eight scales.
+// A k-block of one token on a half warp, 16 elements a lane (past K: zeros)
 template <typename T>
-__device__ __forceinline__ void put_kblock(uint8_t* tile, const mx::Vec8<T>& x, int Bt, int r, int lane) {
-  uint32_t sc;
-  const uint32_t c = mx::quant8<T>(x, sc);
-  *reinterpret_cast<uint32_t*>(tile + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = c;
-  if ((lane & 3) == 0)
-    tile[Bt * (KBW / 2) + (r >> 7) * kSfBytes + (lane >> 4) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 +
-         ((lane >> 2) & 3)] = uint8_t(sc);
+struct KBlock {
+  mx::Vec8<T> h[2];
+};
+template <typename T>
+__device__ __forceinline__ KBlock<T> load_kblock(const T* row, int kb, int K, int lane, bool ok) {
+  KBlock<T> x;
+  const int k = kb * KBW + (lane & 15) * 2 * mx::kVec;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    x.h[h] = ok && k + h * mx::kVec < K ? mx::load8(row + k + h * mx::kVec) : mx::zero8<T>();
+  return x;
 }
 
-// kFuse: the CTA's k-blocks [kb0, kb1) of every token into its tiles at xs
-// (warps w of 4); four (k-block, token) units of a warp in flight
+// ... quantised into row r of a tile of Bt rows: the row's codes and its eight
+// scales (the whole warp calls it; a half with ok false stores nothing)
+template <typename T>
+__device__ __forceinline__ void put_kblock(uint8_t* tile, const KBlock<T>& x, int Bt, int r, int lane, bool ok) {
+  uint32_t sc;
+  const uint2 c = mx::quant16<T>(x.h, sc);
+  if (!ok) return;
+  const int l = lane & 15;
+  *reinterpret_cast<uint2*>(tile + r * 128 + (((l >> 1) ^ (r & 7)) << 4) + (l & 1) * 8) = c;
+  if ((l & 1) == 0)
+    tile[Bt * (KBW / 2) + (r >> 7) * kSfBytes + (l >> 3) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + ((l >> 1) & 3)] =
+        uint8_t(sc);
+}
+
+// kFuse: the CTA's k-blocks [kb0, kb1) of every token into its tiles at xs, a
+// half warp (of 8) a (k-block, token) unit, two units in flight
 template <typename T>
 __device__ __forceinline__ void fill_x(const Args& a, uint8_t* xs, uint32_t x_tile, int kb0, int kb1, int w, int lane) {
   const T* x = reinterpret_cast<const T*>(a.x);
   const int units = (kb1 - kb0) * a.B;
-  constexpr int kFly = 4;
-  for (int u0 = w; u0 < units; u0 += 4 * kFly) {
-    mx::Vec8<T> v[kFly];
+  constexpr int kFly = 2;
+  for (int u0 = 2 * w; u0 < units; u0 += 8 * kFly) {
+    KBlock<T> v[kFly];
     int kb[kFly], b[kFly];
+    bool ok[kFly];
 #pragma unroll
     for (int i = 0; i < kFly; ++i) {
-      const int u = u0 + 4 * i;
+      const int u = u0 + (lane >> 4) + 8 * i;
+      ok[i] = u < units;
       kb[i] = u / a.B;
       b[i] = u - kb[i] * a.B;
-      const int k = (kb0 + kb[i]) * KBW + lane * mx::kVec;
-      v[i] = u < units && k < a.K ? mx::load8(x + b[i] * a.ld_x + k) : mx::zero8<T>();
+      v[i] = load_kblock(x + b[i] * a.ld_x, kb0 + kb[i], a.K, lane, ok[i]);
     }
 #pragma unroll
-    for (int i = 0; i < kFly; ++i)
-      if (u0 + 4 * i < units) put_kblock<T>(xs + kb[i] * x_tile, v[i], a.Bt, b[i], lane);
+    for (int i = 0; i < kFly; ++i) put_kblock<T>(xs + kb[i] * x_tile, v[i], a.Bt, b[i], lane, ok[i]);
   }
 }
 
@@ -514,11 +531,10 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
   }
 }
 
-// X [B, K] -> its tiles.  A warp takes kQuantUnroll k-blocks of one token: its
-// lanes hold the 256 elements of a k-block, so it writes the row's 128 B of
-// codes and eight scales (past K: zeros).
+// X [B, K] -> its tiles.  A warp takes 2 kQuantUnroll k-blocks of one token,
+// a half warp each.
 constexpr int kQuantThreads = 256;
-constexpr int kQuantUnroll = 4;
+constexpr int kQuantUnroll = 2;
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads) quant_x_kernel(const T* __restrict__ x, int64_t ld_x,
                                                                 uint8_t* __restrict__ tiles, int B, int K, int Bt,
@@ -526,25 +542,22 @@ __global__ void __launch_bounds__(kQuantThreads) quant_x_kernel(const T* __restr
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const int runs = (nkb + kQuantUnroll - 1) / kQuantUnroll;  // of a token
+  const int runs = (nkb + 2 * kQuantUnroll - 1) / (2 * kQuantUnroll);  // of a token
   const int64_t total = int64_t(B) * runs, step = int64_t(gridDim.x) * (kQuantThreads / 32);
   for (int64_t w = int64_t(blockIdx.x) * (kQuantThreads / 32) + (threadIdx.x >> 5); w < total; w += step) {
     // (a 64-bit division was a quarter of the instructions)
     const int b = total < (int64_t(1) << 32) ? int(uint32_t(w) / uint32_t(runs)) : int(w / runs);
-    const int kb0 = int(w - int64_t(b) * runs) * kQuantUnroll;
-    const T* src = x + b * ld_x;
-    mx::Vec8<T> x8[kQuantUnroll];
+    const int kb0 = int(w - int64_t(b) * runs) * 2 * kQuantUnroll + (lane >> 4);
+    KBlock<T> v[kQuantUnroll];
 #pragma unroll
-    for (int u = 0; u < kQuantUnroll; ++u) {
-      const int k = (kb0 + u) * KBW + lane * mx::kVec;
-      x8[u] = k < K ? mx::load8(src + k) : mx::zero8<T>();
-    }
+    for (int u = 0; u < kQuantUnroll; ++u)
+      v[u] = load_kblock(x + b * ld_x, kb0 + 2 * u, K, lane, kb0 + 2 * u < nkb);
     const int mt = int(uint32_t(b) / uint32_t(Bt)), r = b - mt * Bt;
     const int tile_bytes = Bt * (KBW / 2) + groups * kSfBytes;
     uint8_t* tile = tiles + (int64_t(mt) * nkb + kb0) * tile_bytes;
 #pragma unroll
     for (int u = 0; u < kQuantUnroll; ++u)
-      if (kb0 + u < nkb) put_kblock<T>(tile + u * tile_bytes, x8[u], Bt, r, lane);  // (the warp's: uniform)
+      put_kblock<T>(tile + 2 * u * tile_bytes, v[u], Bt, r, lane, kb0 + 2 * u < nkb);
   }
 }
 
@@ -833,7 +846,7 @@ extern "C" int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const v
     }
   }
   if (!p.fuse) {
-    const int64_t q_warps = int64_t(B) * ((nkb + lmx::kQuantUnroll - 1) / lmx::kQuantUnroll);
+    const int64_t q_warps = int64_t(B) * ((nkb + 2 * lmx::kQuantUnroll - 1) / (2 * lmx::kQuantUnroll));
     const int per = lmx::kQuantThreads / 32;
     const dim3 qgrid(unsigned(std::min<int64_t>((q_warps + per - 1) / per, int64_t(num_sms()) * 32)));
     auto quant = [&](auto* ptr) {

@@ -117,6 +117,64 @@ __device__ __forceinline__ uint32_t quant8(const Vec8<__nv_bfloat16>& x, uint32_
   return sc == 255u ? 0u : e2m1x8(f);
 }
 
+// The same for 16 consecutive elements a lane, a block on two neighbouring
+// lanes: one shuffle and one scale for twice the elements.  The instructions
+// are what bounds the quantisation of a large activation in L2's reach
+// (4096 x 8192 bf16: 17.4 us with 8 a lane, 12.3 with the loads and stores
+// alone).
+template <typename T>
+__device__ __forceinline__ uint2 quant16(const Vec8<T> (&x)[2], uint32_t& sc) {
+  float v[2 * kVec];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (sizeof(T) == 4) {
+      const uint32_t w[8] = {x[h].w[0].x, x[h].w[0].y, x[h].w[0].z, x[h].w[0].w,
+                             x[h].w[1].x, x[h].w[1].y, x[h].w[1].z, x[h].w[1].w};
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) v[kVec * h + i] = __uint_as_float(w[i]);
+    } else {
+      const __half2* p = reinterpret_cast<const __half2*>(&x[h].w[0]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(p[i]);
+        v[kVec * h + 2 * i] = f.x;
+        v[kVec * h + 2 * i + 1] = f.y;
+      }
+    }
+  }
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 2 * kVec; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  const int field = int(m >> 23);
+  sc = field == 255 ? 255u : uint32_t(max(field - 2, 0));
+  const float inv = __uint_as_float((254u - sc) << 23);
+#pragma unroll
+  for (int i = 0; i < 2 * kVec; ++i) v[i] *= inv;
+  return sc == 255u ? make_uint2(0, 0) : make_uint2(e2m1x8(v), e2m1x8(v + kVec));
+}
+template <>
+__device__ __forceinline__ uint2 quant16(const Vec8<__nv_bfloat16> (&x)[2], uint32_t& sc) {
+  const uint32_t w[8] = {x[0].w[0].x, x[0].w[0].y, x[0].w[0].z, x[0].w[0].w,
+                         x[1].w[0].x, x[1].w[0].y, x[1].w[0].z, x[1].w[0].w};
+  __nv_bfloat162 m = __habs2(as_bf162(w[0]));
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(as_bf162(w[i])));
+  m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  const uint32_t mb = as_u32(m);
+  const int field = int(max((mb >> 7) & 0xffu, (mb >> 23) & 0xffu));
+  sc = field == 255 ? 255u : uint32_t(max(field - 2, 0));
+  const __nv_bfloat162 inv = as_bf162(((254u - sc) << 7) * 0x10001u);
+  float f[2 * kVec];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t y = as_u32(__hmul2(as_bf162(w[i]), inv));
+    f[2 * i] = __uint_as_float(y << 16);
+    f[2 * i + 1] = __uint_as_float(y & 0xffff0000u);
+  }
+  return sc == 255u ? make_uint2(0, 0) : make_uint2(e2m1x8(f), e2m1x8(f + kVec));
+}
+
 // the values the codes stand for
 __device__ __forceinline__ void values8(uint32_t codes, uint32_t sc, float* v) {
   const float s = sc == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(sc ? sc << 23 : 0x00400000u);
