@@ -68,7 +68,7 @@ constexpr int kMaxSplit = 16;
 constexpr int THREADS = 224;
 constexpr int kSmemBytes = 232448;
 constexpr int kAuxBytes = 256;
-constexpr int kFuseUnits = 32;                  // (token, k-block) units of X a CTA quantises itself, at most
+constexpr int kFuseUnits = 48;                  // (token, k-block) units of X a CTA quantises itself, at most
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColSf = 2 * kMaxBt;         // scales of each stage: 8 columns of W, 8 a group of X
 __host__ __device__ constexpr int sf_cols(int groups) { return 8 + 8 * groups; }
@@ -179,10 +179,11 @@ __device__ __forceinline__ KBlock<T> load_kblock(const T* row, int kb, int K, in
 template <typename T>
 __device__ __forceinline__ void put_kblock(uint8_t* tile, const KBlock<T>& x, int Bt, int r, int lane, bool ok) {
   uint32_t sc;
-  const uint2 c = mx::quant16<T>(x.h, sc);
+  uint32_t c[2];
+  mx::quant(x.h, sc, c);
   if (!ok) return;
   const int l = lane & 15;
-  *reinterpret_cast<uint2*>(tile + r * 128 + (((l >> 1) ^ (r & 7)) << 4) + (l & 1) * 8) = c;
+  *reinterpret_cast<uint2*>(tile + r * 128 + (((l >> 1) ^ (r & 7)) << 4) + (l & 1) * 8) = make_uint2(c[0], c[1]);
   if ((l & 1) == 0)
     tile[Bt * (KBW / 2) + (r >> 7) * kSfBytes + (l >> 3) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + ((l >> 1) & 3)] =
         uint8_t(sc);
@@ -719,10 +720,9 @@ static Plan pick_plan(int B, int N, int nkb) {
   }
   // Quantising X in the product saves a launch and X's way through memory and
   // costs each CTA its share of X on four warps.  Measured, fused against two
-  // launches: 1 x 1024 x 4096 (2 units a CTA) 4.8 / 5.8 us, 8 x 1024 x 4096
-  // (16) 5.8 / 6.5, 12 x 1024 x 4096 (24) 6.4 / 6.4, 8 x 32768 x 1024 (32) 6.9 /
-  // 6.8, 16 x 1024 x 4096 (32) 6.9 / 6.5, 24 x 1024 x 4096 (48) 7.9 / 6.7; a
-  // launch more is ~5 us of the host's time, hence 32.
+  // launches: 1 x 1024 x 4096 (2 units a CTA) 4.8 / 5.7 us, 8 x 1024 x 4096
+  // (16) 5.4 / 6.2, 16 x 1024 x 4096 (32) 6.1 / 6.4, 12 x 32768 x 1024 (48) 6.6 /
+  // 6.8, 24 x 1024 x 4096 (48) 6.8 / 6.5, 16 x 32768 x 1024 (64) 7.2 / 6.8.
   const int share = (nkb + best.split - 1) / best.split;
   if (best.m_tiles == 1 && int64_t(share) * B <= kFuseUnits) {
     Plan f = best;

@@ -21,7 +21,7 @@ namespace dsa {
 namespace mx {
 
 constexpr int kBlock = 32;
-constexpr int kVec = 8;  // elements a lane holds; a block is 4 neighbouring lanes
+constexpr int kVec = 8;  // a lane's elements come in eights
 
 // A lane's 8 consecutive elements as they lie in memory.
 template <typename T>
@@ -60,119 +60,78 @@ __device__ __forceinline__ uint32_t e2m1x8(const float* f) {
   return c;
 }
 
-// Scale code of the block that this lane and its three neighbours hold (every
-// lane of the warp calls it) and this lane's 8 elements as E2M1 codes.
+// A block on 4 / H neighbouring lanes, H eights each: its scale code (every
+// lane of the warp calls it) and the E2M1 codes of this lane's eights.  With
+// one eight a lane the shuffles and the scale's arithmetic bound 16-bit
+// inputs, not the bytes (4096 x 8192 bf16 into the projection's tiles: 17.4
+// us; loads and stores alone 12.3).
 // fp32 and fp16: the fp32 bits without the sign order as integers, NaN and
 // infinity above every number.
-template <typename T>
-__device__ __forceinline__ uint32_t quant8(const Vec8<T>& x, uint32_t& sc) {
-  float v[kVec];
-  if constexpr (sizeof(T) == 4) {
-    const uint32_t w[8] = {x.w[0].x, x.w[0].y, x.w[0].z, x.w[0].w, x.w[1].x, x.w[1].y, x.w[1].z, x.w[1].w};
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] = __uint_as_float(w[i]);
-  } else {
-    const __half2* h = reinterpret_cast<const __half2*>(&x.w[0]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(h[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
-  }
+template <typename T, int H>
+__device__ __forceinline__ void quant(const Vec8<T> (&x)[H], uint32_t& sc, uint32_t (&codes)[H]) {
+  float v[H][kVec];
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  const int field = int(m >> 23);
-  sc = field == 255 ? 255u : uint32_t(max(field - 2, 0));
-  const float inv = __uint_as_float((254u - sc) << 23);
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) v[i] *= inv;
-  return sc == 255u ? 0u : e2m1x8(v);
-}
-// bf16: maximum and scaling two elements an instruction (a power of two, so
-// exact where the code is not zero); the quantisation of a 4096 x 8192
-// activation is bound by instructions, not bytes.
-template <>
-__device__ __forceinline__ uint32_t quant8(const Vec8<__nv_bfloat16>& x, uint32_t& sc) {
-  const uint32_t w[4] = {x.w[0].x, x.w[0].y, x.w[0].z, x.w[0].w};
-  __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(as_bf162(w[0])), __habs2(as_bf162(w[1]))),
-                                 __hmax2_nan(__habs2(as_bf162(w[2])), __habs2(as_bf162(w[3]))));
-  m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  const uint32_t mb = as_u32(m);
-  // the exponent field orders as the number does, NaN and infinity 255
-  const int field = int(max((mb >> 7) & 0xffu, (mb >> 23) & 0xffu));
-  sc = field == 255 ? 255u : uint32_t(max(field - 2, 0));
-  const __nv_bfloat162 inv = as_bf162(((254u - sc) << 7) * 0x10001u);
-  float f[kVec];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t y = as_u32(__hmul2(as_bf162(w[i]), inv));
-    f[2 * i] = __uint_as_float(y << 16);
-    f[2 * i + 1] = __uint_as_float(y & 0xffff0000u);
-  }
-  return sc == 255u ? 0u : e2m1x8(f);
-}
-
-// The same for 16 consecutive elements a lane, a block on two neighbouring
-// lanes: one shuffle and one scale for twice the elements.  The instructions
-// are what bounds the quantisation of a large activation in L2's reach
-// (4096 x 8192 bf16: 17.4 us with 8 a lane, 12.3 with the loads and stores
-// alone).
-template <typename T>
-__device__ __forceinline__ uint2 quant16(const Vec8<T> (&x)[2], uint32_t& sc) {
-  float v[2 * kVec];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < H; ++h) {
     if constexpr (sizeof(T) == 4) {
       const uint32_t w[8] = {x[h].w[0].x, x[h].w[0].y, x[h].w[0].z, x[h].w[0].w,
                              x[h].w[1].x, x[h].w[1].y, x[h].w[1].z, x[h].w[1].w};
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) v[kVec * h + i] = __uint_as_float(w[i]);
+      for (int i = 0; i < kVec; ++i) v[h][i] = __uint_as_float(w[i]);
     } else {
       const __half2* p = reinterpret_cast<const __half2*>(&x[h].w[0]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 f = __half22float2(p[i]);
-        v[kVec * h + 2 * i] = f.x;
-        v[kVec * h + 2 * i + 1] = f.y;
+        v[h][2 * i] = f.x;
+        v[h][2 * i + 1] = f.y;
       }
     }
-  }
-  uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 2 * kVec; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    for (int i = 0; i < kVec; ++i) m = max(m, __float_as_uint(v[h][i]) & 0x7fffffffu);
+  }
+#pragma unroll
+  for (int o = 1; o < 4 / H; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   const int field = int(m >> 23);
   sc = field == 255 ? 255u : uint32_t(max(field - 2, 0));
   const float inv = __uint_as_float((254u - sc) << 23);
 #pragma unroll
-  for (int i = 0; i < 2 * kVec; ++i) v[i] *= inv;
-  return sc == 255u ? make_uint2(0, 0) : make_uint2(e2m1x8(v), e2m1x8(v + kVec));
-}
-template <>
-__device__ __forceinline__ uint2 quant16(const Vec8<__nv_bfloat16> (&x)[2], uint32_t& sc) {
-  const uint32_t w[8] = {x[0].w[0].x, x[0].w[0].y, x[0].w[0].z, x[0].w[0].w,
-                         x[1].w[0].x, x[1].w[0].y, x[1].w[0].z, x[1].w[0].w};
-  __nv_bfloat162 m = __habs2(as_bf162(w[0]));
+  for (int h = 0; h < H; ++h) {
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(as_bf162(w[i])));
-  m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    for (int i = 0; i < kVec; ++i) v[h][i] *= inv;
+    codes[h] = sc == 255u ? 0u : e2m1x8(v[h]);
+  }
+}
+// bf16: maximum and scaling two elements an instruction (a power of two, so
+// exact where the code is not zero)
+template <int H>
+__device__ __forceinline__ void quant(const Vec8<__nv_bfloat16> (&x)[H], uint32_t& sc, uint32_t (&codes)[H]) {
+  __nv_bfloat162 m = as_bf162(0u);
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    const uint32_t w[4] = {x[h].w[0].x, x[h].w[0].y, x[h].w[0].z, x[h].w[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __hmax2_nan(m, __habs2(as_bf162(w[i])));
+  }
+#pragma unroll
+  for (int o = 1; o < 4 / H; o <<= 1) m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   const uint32_t mb = as_u32(m);
+  // the exponent field orders as the number does, NaN and infinity 255
   const int field = int(max((mb >> 7) & 0xffu, (mb >> 23) & 0xffu));
   sc = field == 255 ? 255u : uint32_t(max(field - 2, 0));
   const __nv_bfloat162 inv = as_bf162(((254u - sc) << 7) * 0x10001u);
-  float f[2 * kVec];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t y = as_u32(__hmul2(as_bf162(w[i]), inv));
-    f[2 * i] = __uint_as_float(y << 16);
-    f[2 * i + 1] = __uint_as_float(y & 0xffff0000u);
+  for (int h = 0; h < H; ++h) {
+    const uint32_t w[4] = {x[h].w[0].x, x[h].w[0].y, x[h].w[0].z, x[h].w[0].w};
+    float f[kVec];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t y = as_u32(__hmul2(as_bf162(w[i]), inv));
+      f[2 * i] = __uint_as_float(y << 16);
+      f[2 * i + 1] = __uint_as_float(y & 0xffff0000u);
+    }
+    codes[h] = sc == 255u ? 0u : e2m1x8(f);
   }
-  return sc == 255u ? make_uint2(0, 0) : make_uint2(e2m1x8(f), e2m1x8(f + kVec));
 }
 
 // the values the codes stand for
