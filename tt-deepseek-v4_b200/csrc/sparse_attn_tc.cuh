@@ -62,6 +62,14 @@
 // the copies of the bf16 cache land; everything behind the tile is the same.
 // Registers, not a staging ring: the three 64 KB slots leave 5 KB of shared
 // memory.  As a warp stores a row of tile t it requests its row of t + 1.
+// Measured at 64 sequences x 2176 rows: 41.0 us (bf16 rows 34.8).  A tile takes
+// ~3.3K cycles: a slot is held ~2.2K while it is filled, then as long as a copied
+// one (S, softmax, PV), and three slots cover that round trip.  Expanding 8
+// dims takes 20 conversions and products a lane; without it (rows stored as
+// they come, wrong results) the kernel takes 36.8.  9 producer warps in 512
+// threads 54.5; 17 in 768 (80 registers, spills) 49.9; the tile expanded in
+// registers before its slot is free 45.9-48.9 (two rows in flight, or the next
+// rows requested only after the stores), two of the five rows so 40.8.
 //
 // Every mbarrier wait is bounded (about a second); a wait that runs out sets
 // a status bit and an abort flag that makes all later waits of the CTA return
