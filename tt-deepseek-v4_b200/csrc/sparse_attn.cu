@@ -30,7 +30,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // (M, L, sum_p o_p e^{m_p-M}) without the sink.  One warp per (query row,
 // head, slice of DPL * 32 output dims): the split statistics are reduced
 // across lanes (any number of splits), then lane l combines DPL dims of
-// every split, four splits' loads in flight at a time.  DPL = 16 covers the
+// every split, eight splits' loads in flight at a time.  DPL = 16 covers the
 // 512 dims with one warp (many query rows); DPL = 4 spreads a row over 4x
 // more warps for the few-row case (a single long context), where the
 // combine would otherwise run on M * 8 CTAs.
@@ -64,36 +64,47 @@ __global__ void __launch_bounds__(32 * kCombineWarps) lse_combine_kernel(
   float acc[DPL];
 #pragma unroll
   for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int p = 0; p < P; ++p) {
-    const float mp = ml(p, 0);
-    float w = (mp == -INFINITY) ? 0.f : expf(mp - Mx);
-    const int64_t off = int64_t(p) * o_ps + (int64_t(m) * H + h) * D + d0;
-    if constexpr (kNormBF16) {
-      w *= ml(p, 1);
-      // DPL bf16 values = DPL / 4 8-byte words
-      const uint2* src = reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(part_o) + off);
-      uint2 v[DPL / 4];
+  // Lane p of a group of 32 splits works out its weight, the loop takes it by a
+  // shuffle: only the partials' loads are left in it, eight splits in flight
+  // (a weight in every lane, four in flight: 17.1 us for one row's attention
+  // over 17 splits and their combine, now 15.5; the same sums in the same order).
+  for (int p0 = 0; p0 < P; p0 += 32) {
+    float wl = 0.f;
+    if (p0 + lane < P) {
+      const float mp = ml(p0 + lane, 0);
+      wl = (mp == -INFINITY) ? 0.f : expf(mp - Mx);
+      if constexpr (kNormBF16) wl *= ml(p0 + lane, 1);
+    }
+    const int n = min(32, P - p0);
+#pragma unroll 8
+    for (int q = 0; q < n; ++q) {
+      const float w = __shfl_sync(0xffffffffu, wl, q);
+      const int64_t off = int64_t(p0 + q) * o_ps + (int64_t(m) * H + h) * D + d0;
+      if constexpr (kNormBF16) {
+        // DPL bf16 values = DPL / 4 8-byte words
+        const uint2* src = reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(part_o) + off);
+        uint2 v[DPL / 4];
 #pragma unroll
-      for (int i = 0; i < DPL / 4; ++i) v[i] = __ldg(src + i);
+        for (int i = 0; i < DPL / 4; ++i) v[i] = __ldg(src + i);
 #pragma unroll
-      for (int i = 0; i < DPL / 4; ++i) {
-        acc[4 * i + 0] = fmaf(w, __uint_as_float(v[i].x << 16), acc[4 * i + 0]);
-        acc[4 * i + 1] = fmaf(w, __uint_as_float(v[i].x & 0xffff0000u), acc[4 * i + 1]);
-        acc[4 * i + 2] = fmaf(w, __uint_as_float(v[i].y << 16), acc[4 * i + 2]);
-        acc[4 * i + 3] = fmaf(w, __uint_as_float(v[i].y & 0xffff0000u), acc[4 * i + 3]);
-      }
-    } else {
-      const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(part_o) + off);
-      float4 v[DPL / 4];
+        for (int i = 0; i < DPL / 4; ++i) {
+          acc[4 * i + 0] = fmaf(w, __uint_as_float(v[i].x << 16), acc[4 * i + 0]);
+          acc[4 * i + 1] = fmaf(w, __uint_as_float(v[i].x & 0xffff0000u), acc[4 * i + 1]);
+          acc[4 * i + 2] = fmaf(w, __uint_as_float(v[i].y << 16), acc[4 * i + 2]);
+          acc[4 * i + 3] = fmaf(w, __uint_as_float(v[i].y & 0xffff0000u), acc[4 * i + 3]);
+        }
+      } else {
+        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(part_o) + off);
+        float4 v[DPL / 4];
 #pragma unroll
-      for (int i = 0; i < DPL / 4; ++i) v[i] = __ldg(src + i);
+        for (int i = 0; i < DPL / 4; ++i) v[i] = __ldg(src + i);
 #pragma unroll
-      for (int i = 0; i < DPL / 4; ++i) {
-        acc[4 * i + 0] = fmaf(w, v[i].x, acc[4 * i + 0]);
-        acc[4 * i + 1] = fmaf(w, v[i].y, acc[4 * i + 1]);
-        acc[4 * i + 2] = fmaf(w, v[i].z, acc[4 * i + 2]);
-        acc[4 * i + 3] = fmaf(w, v[i].w, acc[4 * i + 3]);
+        for (int i = 0; i < DPL / 4; ++i) {
+          acc[4 * i + 0] = fmaf(w, v[i].x, acc[4 * i + 0]);
+          acc[4 * i + 1] = fmaf(w, v[i].y, acc[4 * i + 1]);
+          acc[4 * i + 2] = fmaf(w, v[i].z, acc[4 * i + 2]);
+          acc[4 * i + 3] = fmaf(w, v[i].w, acc[4 * i + 3]);
+        }
       }
     }
   }
