@@ -430,3 +430,21 @@ def test_captured_steps_and_a_second_stream(cuda_dev):
         assert torch.equal(out, ops.sparse_attn(q, rows_bf, idx, sink, SCALE))
         assert torch.equal(_bits(back), _bits(ops.kv_quant_read(ref, idx[:, 0].contiguous())))
         assert all(torch.equal(e, want2) for e in eager)
+
+
+def test_refusals_of_sizes_and_types_that_do_not_fit(cuda_dev):
+    from dsv4attn import ops
+    d = cuda_dev
+    cache = ops.kv_quant_cache(2, 8, device=d)
+    kv = torch.zeros(2, 512, dtype=BF, device=d)
+    pos = torch.zeros(2, dtype=I32, device=d)
+    for win in (2**32 + 8, -2**32 + 8):                    # 8 in 32 bits
+        with pytest.raises(ValueError, match="too large"):
+            ops.kv_quant_write(kv, cache, pos, win)
+    with pytest.raises(ValueError, match="status must be torch.int32"):
+        ops.kv_quant_read(cache, status=torch.zeros(1, dtype=torch.int64, device=d))
+    with pytest.raises(ValueError, match="tensors on cuda:0 and cpu"):
+        ops.kv_quant_read(cache, status=torch.zeros(1, dtype=I32))
+    with pytest.raises(TypeError, match="out"):
+        ops.mxfp4_quant(kv, out=False)
+    assert not cache.any()

@@ -193,3 +193,12 @@ def test_linear_mxfp4_refusals():
     assert call(wsb=100, **big) == _lib.DSA_ERR_WORKSPACE and "workspace" in _lib.last_error()
     assert call(ws=None, **big) == _lib.DSA_ERR_WORKSPACE
     assert call(B=0) == _lib.DSA_OK
+
+
+def test_a_missing_module_is_an_error(monkeypatch):
+    import sys
+    from dsv4attn import _lib
+    monkeypatch.setitem(sys.modules, "dsv4attn._torch_ops", None)
+    monkeypatch.delattr("dsv4attn._torch_ops", raising=False)
+    with pytest.raises(_lib.NativeLibraryError, match="build.py"):
+        _lib.torch_ops()

@@ -5,8 +5,10 @@
 Compiles every ``csrc/*.cu`` with nvcc for ``sm_100a`` (no PTX for other
 architectures, no JIT) and links one shared library against the shared
 CUDA runtime, so the process that loads it through ctypes shares one
-runtime (and one primary context) with PyTorch.  Objects are rebuilt only
-when a source or header is newer than the library.
+runtime (and one primary context) with PyTorch.  ``csrc/torch_ops.cpp`` (the
+low-bit operators over torch tensors) becomes ``dsv4attn/_torch_ops.so``, a
+Python module linked against that library and torch.  Objects are rebuilt
+only when a source or header is newer than the library.
 """
 
 from __future__ import annotations
@@ -17,12 +19,15 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OUT_DIR = os.path.join(HERE, "dsv4attn")
 LIB = os.path.join(OUT_DIR, "libdsv4attn.so")
+TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
+TORCH_LIB = os.path.join(OUT_DIR, "_torch_ops.so")
 OBJ_DIR = os.path.join(HERE, "_build")
 
 GENCODE = "-gencode=arch=compute_100a,code=sm_100a"
@@ -52,8 +57,35 @@ def needs_build() -> bool:
     return any(os.path.getmtime(p) > t for p in _sources() + _headers() + [__file__])
 
 
+def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
+    """The Python module over torch tensors (needs the library built)."""
+    deps = [TORCH_SRC, __file__] + glob.glob(os.path.join(INCLUDE, "*.h"))
+    if not force and os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) > max(map(os.path.getmtime, deps)):
+        return TORCH_LIB
+    import torch
+    tdir = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(find_nvcc())))
+    inc = [os.path.join(tdir, "include"), os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
+           os.path.join(cuda, "include"), sysconfig.get_paths()["include"], INCLUDE]
+    tmp = TORCH_LIB + ".tmp"
+    # the g++ that nvcc compiles the host side with, not $CXX: one that links
+    # its own static libstdc++ gives the process a second C++ runtime, and an
+    # exception that crosses into torch's ends it
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f for i in inc for f in ("-isystem", i)), TORCH_SRC, "-o", tmp, "-L" + OUT_DIR, "-l:libdsv4attn.so",
+           "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(tdir, "lib"), "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+           "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> str:
     if not force and not needs_build():
+        build_torch_ops(verbose=verbose)
         return LIB
     nvcc = find_nvcc()
     os.makedirs(OBJ_DIR, exist_ok=True)
@@ -76,6 +108,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
+    build_torch_ops(force=force, verbose=verbose)
     return LIB
 
 

@@ -131,6 +131,18 @@ def lib():
     return _lib
 
 
+def torch_ops():
+    """The compiled module of the low-bit operators (csrc/torch_ops.cpp),
+    loaded next to the library; raises if it is absent."""
+    lib()
+    try:
+        from . import _torch_ops
+    except ImportError as e:
+        raise NativeLibraryError(f"dsv4attn._torch_ops cannot be loaded ({e}); "
+                                 "build it with `python tt-deepseek-v4_b200/build.py`") from e
+    return _torch_ops
+
+
 def last_error() -> str:
     msg = lib().dsa_last_error()
     return msg.decode() if msg else ""

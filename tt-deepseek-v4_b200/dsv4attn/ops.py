@@ -48,6 +48,17 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+_native_ops = None
+
+
+def _native():
+    """The compiled low-bit operators (loaded once)."""
+    global _native_ops
+    if _native_ops is None:
+        _native_ops = _lib.torch_ops()
+    return _native_ops
+
+
 class Workspace:
     """Grow-only per-device scratch buffer owned by the caller (allocate it
     before CUDA-graph capture; the native calls never allocate)."""
@@ -220,7 +231,8 @@ def pack_linear_weight_mxfp4(codes: torch.Tensor, scales: torch.Tensor | None = 
         _, scales, codes = mxfp4_quant(codes)
     _need(scales, "scales")
     if codes.dtype not in (torch.uint8, torch.int8, torch.float4_e2m1fn_x2) or codes.dim() != 2:
-        raise ValueError(f"codes must be [N, K/2] uint8, int8 or float4_e2m1fn_x2, got {codes.dtype} {tuple(codes.shape)}")
+        raise ValueError(f"codes must be [N, K/2] uint8, int8 or float4_e2m1fn_x2, got {codes.dtype} "
+                         f"{tuple(codes.shape)}")
     if scales.dtype not in (torch.uint8, torch.float8_e8m0fnu):
         raise ValueError(f"scales must be uint8 or float8_e8m0fnu, got {scales.dtype}")
     _contig(codes, "codes")
@@ -229,13 +241,15 @@ def pack_linear_weight_mxfp4(codes: torch.Tensor, scales: torch.Tensor | None = 
     if tuple(scales.shape) != (N, K // 32) or K % 32:
         raise ValueError(f"scales {tuple(scales.shape)} do not match codes {tuple(codes.shape)}: [N, K/32] for K a "
                          "multiple of 32")
-    stream = _launch_stream(codes, scales)
+    if codes.device != scales.device or codes.get_device() != torch.cuda.current_device():
+        raise ValueError(f"codes on {codes.device}, scales on {scales.device}, current device is "
+                         f"cuda:{torch.cuda.current_device()}")
     nbytes = lib().dsa_linear_mxfp4_packed_bytes(N, K)
     if nbytes == 0:
         raise ValueError(f"weight [{N}, {K}]: sizes must be positive and at most 2^24")
     packed = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
-    check(lib().dsa_linear_mxfp4_pack(codes.data_ptr(), scales.data_ptr(), N, K, packed.data_ptr(), nbytes, stream),
-          "linear_mxfp4_pack")
+    check(lib().dsa_linear_mxfp4_pack(codes.data_ptr(), scales.data_ptr(), N, K, packed.data_ptr(), nbytes,
+                                      _stream(codes)), "linear_mxfp4_pack")
     return MXFP4Weight(packed, N, K)
 
 
@@ -247,34 +261,9 @@ def linear_mxfp4(x: torch.Tensor, w: MXFP4Weight, out: torch.Tensor | None = Non
     bf16, or the fp32 sums with ``out_f32``.  Without ``ws`` the scratch (x's
     codes and scales, where the product does not quantise x itself) is
     allocated on the current stream for this call."""
-    _need(x, "x")
-    x_type = _X_TYPES.get(x.dtype)
-    if x_type is None:
-        raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
     if not isinstance(w, MXFP4Weight):
         raise TypeError("w must be an MXFP4Weight (pack_linear_weight_mxfp4)")
-    N, K = w.N, w.K
-    if x.dim() != 2 or x.shape[1] != K or x.stride(1) != 1:
-        raise ValueError(f"x must be [B, {K}] with contiguous rows, got {tuple(x.shape)}")
-    B = x.shape[0]
-    dtype = F32 if out_f32 else BF16
-    stream = _launch_stream(x, w.packed, out, status)
-    if out is None:
-        out = torch.empty((B, N), dtype=dtype, device=x.device)
-    else:
-        _need(out, "out", dtype)
-        if out.dim() != 2 or out.shape[0] != B or out.shape[1] < N or out.stride(1) != 1:
-            raise ValueError(f"out must be [{B}, >={N}] with contiguous rows, got {tuple(out.shape)}")
-    if B == 0:
-        return out
-    need = _linear_ws[x.get_device(), B, N, K]
-    buf = None
-    if need:
-        buf = ws.get(need) if ws is not None else torch.empty(need, dtype=_U8, device=x.device)
-    check(lib().dsa_linear_mxfp4(x.data_ptr(), x_type, x.stride(0), w.packed.data_ptr(), out.data_ptr(),
-                                 out.stride(0), B, N, K, out_f32, None if buf is None else buf.data_ptr(), need,
-                                 None if status is None else status.data_ptr(), stream), "linear_mxfp4")
-    return out
+    return _native().linear_mxfp4(x, w.packed, w.N, w.K, out, out_f32, ws, status)
 
 
 # ------------------------------------------------------------------ attn.kv
@@ -306,59 +295,7 @@ def act_quant_block(x: torch.Tensor, block: int = 64, fp8_max: float = 448.0, ep
     return out, scales, codes
 
 
-class _Sizes(dict):
-    """Workspace sizes already asked for, by shape and device: host arithmetic
-    of the library that a call would repeat (0.1 against 0.8 us)."""
-
-    def __init__(self, ask):
-        super().__init__()
-        self.ask = ask
-
-    def __missing__(self, key):
-        if len(self) >= 4096:
-            self.clear()
-        n = self[key] = int(self.ask(*key[1:]))
-        return n
-
-
-_linear_ws = _Sizes(lambda B, N, K: lib().dsa_linear_mxfp4_workspace_size(B, N, K))
-_attn_ws = _Sizes(lambda B, S, K: lib().dsa_sparse_attn_workspace_size(B, S, 64, 512, K))
-
 _X_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_U8 = torch.uint8
-
-
-def _row_stride(t: torch.Tensor, name: str) -> int:
-    """Row stride of t [..., K] read as a matrix of rows with unit stride in
-    the last dim."""
-    if t.is_contiguous():
-        return t.shape[-1]
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{name} must have a unit stride in the last dim")
-    try:
-        t2 = t.view(-1, t.shape[-1])
-    except RuntimeError:
-        raise ValueError(f"{name} {tuple(t.shape)} with strides {t.stride()} is not a matrix of rows") from None
-    return t2.stride(0) if t2.shape[0] > 1 else t2.shape[1]
-
-
-def _launch_stream(t: torch.Tensor, *others) -> int:
-    """The current stream of t's device.  Launches go to the current device:
-    t and the other tensors must be on it."""
-    dev = t.get_device()
-    for o in others:
-        if o is not None and o.get_device() != dev:
-            raise ValueError(f"tensors on {t.device} and {o.device}")
-    if dev != torch.cuda.current_device():
-        raise ValueError(f"tensor on {t.device}, current device is cuda:{torch.cuda.current_device()}")
-    return _raw_stream(dev)
-
-
-def _mx_field(t: torch.Tensor, name: str, shape: tuple) -> None:
-    _need(t, name, torch.uint8)
-    _contig(t, name)
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
 
 
 def mxfp4_quant(x: torch.Tensor, out=None, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None):
@@ -368,52 +305,12 @@ def mxfp4_quant(x: torch.Tensor, out=None, codes: torch.Tensor | None = None, sc
     act_quant_block: codes [..., K/2] uint8 (the even element in the low
     half), scales [..., K/32] uint8, and the round-trip values in x's type
     when ``out`` is True or a tensor (which may be x), else None."""
-    _need(x, "x")
-    dtype = x.dtype
-    x_type = _X_TYPES.get(dtype)
-    if x_type is None:
-        raise ValueError(f"x must be bfloat16, float16 or float32, got {dtype}")
-    lead, K = x.shape[:-1], x.shape[-1] if x.dim() else 0
-    if K == 0 or K % 32:
-        raise ValueError(f"last dim {K} must be a positive multiple of 32")
-    ld, ld_out, o_ptr = _row_stride(x, "x"), 0, None
-    stream = _launch_stream(x, None if out is True else out, codes, scales)
-    if out is True:
-        out = torch.empty_like(x) if ld == K else x.new_empty(x.shape)
-        ld_out, o_ptr = K, out.data_ptr()
-    elif out is not None:
-        _need(out, "out", dtype)
-        if out.shape != x.shape:
-            raise ValueError("out must have x's shape")
-        ld_out, o_ptr = _row_stride(out, "out"), out.data_ptr()
-    if codes is None:
-        codes = torch.empty(lead + (K // 2,), dtype=_U8, device=x.device)
-    else:
-        _mx_field(codes, "codes", lead + (K // 2,))
-    if scales is None:
-        scales = torch.empty(lead + (K // 32,), dtype=_U8, device=x.device)
-    else:
-        _mx_field(scales, "scales", lead + (K // 32,))
-    M = x.numel() // K
-    if M:
-        check(lib().dsa_mxfp4_quant(x.data_ptr(), x_type, ld, o_ptr, ld_out, codes.data_ptr(), scales.data_ptr(), M, K,
-                                    stream), "mxfp4_quant")
-    return out, scales, codes
-
-
-_row_bytes: dict = {}  # (D, rope_dim) -> bytes, the sizes in use
+    return _native().mxfp4_quant(x, out, codes, scales)
 
 
 def kv_quant_row_bytes(D: int = 512, rope_dim: int = 64) -> int:
     """Bytes of one record of the FP8 latent cache (608 for 448 + 64 dims)."""
-    n = _row_bytes.get((D, rope_dim))
-    if n is None:
-        n = int(lib().dsa_kv_quant_row_bytes(D, rope_dim))
-        if n == 0:
-            raise ValueError(f"D={D}, rope_dim={rope_dim}: D - rope_dim must be a positive multiple of 64, rope_dim a "
-                             "multiple of 8, D <= 8192")
-        _row_bytes[D, rope_dim] = n
-    return n
+    return _native().kv_quant_row_bytes(D, rope_dim)
 
 
 def kv_quant_cache(B: int, rows: int, D: int = 512, rope_dim: int = 64, device=None) -> torch.Tensor:
@@ -425,31 +322,7 @@ def kv_quant_cache(B: int, rows: int, D: int = 512, rope_dim: int = 64, device=N
 def kv_quant_views(cache: torch.Tensor, D: int = 512, rope_dim: int = 64):
     """``(codes, rope, scales)`` of a cache as views: [..., D - rope_dim]
     float8_e4m3fn, [..., rope_dim] bf16, [..., (D - rope_dim)/64] fp32."""
-    if cache.dtype != torch.uint8 or cache.shape[-1] != kv_quant_row_bytes(D, rope_dim):
-        raise ValueError(f"cache must be uint8 with records of {kv_quant_row_bytes(D, rope_dim)} bytes")
-    a = D - rope_dim
-    b = a + 2 * rope_dim
-    codes, rope, scales, _ = cache.split((a, b - a, a // 16, cache.shape[-1] - b - a // 16), -1)
-    return codes.view(torch.float8_e4m3fn), rope.view(BF16), scales.view(F32)
-
-
-def _quant_cache(cache: torch.Tensor, B: int, D: int, rope_dim: int) -> None:
-    _need(cache, "cache", _U8)
-    rb = kv_quant_row_bytes(D, rope_dim)
-    if cache.dim() == 3:
-        n, rows, width = cache.shape
-        _, row, one = cache.stride()
-        if n >= B and rows >= 1 and width == rb and one == 1 and (row == rb or rows == 1):
-            return
-    raise ValueError(f"cache must be [>={B}, rows, {rb}] with contiguous rows (D={D}, rope_dim={rope_dim}), "
-                     f"got {tuple(cache.shape)}")
-
-
-def _per_sequence(t, name: str, B: int) -> None:
-    _need(t, name, I32)
-    _contig(t, name)
-    if t.numel() != B:
-        raise ValueError(f"{name} has {t.numel()} entries, expected {B}")
+    return _native().kv_quant_views(cache, D, rope_dim)
 
 
 def kv_quant_write(kv: torch.Tensor, cache: torch.Tensor, pos: torch.Tensor, win: int, offset: int = 0,
@@ -460,22 +333,7 @@ def kv_quant_write(kv: torch.Tensor, cache: torch.Tensor, pos: torch.Tensor, win
     to row ``offset + (pos[b] + s) % win``.  n_valid [B] int32: tokens of each
     sequence in a padded batch.  Of more than ``win`` tokens the last ``win``
     are written; every other row stays as it was."""
-    _need(kv, "kv", BF16)
-    if kv.dim() == 2:
-        kv = kv.unsqueeze(1)
-    if kv.dim() != 3 or kv.stride(2) != 1:
-        raise ValueError("kv must be [B, S, D] or [B, D] with a unit stride in the last dim")
-    B, S, D = kv.shape
-    ld_b, ld_s, _ = kv.stride()
-    _quant_cache(cache, B, D, rope_dim)
-    _per_sequence(pos, "pos", B)
-    if n_valid is not None:
-        _per_sequence(n_valid, "n_valid", B)
-    stream = _launch_stream(kv, cache, pos, n_valid)
-    if B and S:
-        check(lib().dsa_kv_quant_write(kv.data_ptr(), ld_b, ld_s, cache.data_ptr(), cache.stride(0), cache.shape[1],
-                                       pos.data_ptr(), _ptr(n_valid), B, S, D, rope_dim, win, offset, stream),
-              "kv_quant_write")
+    _native().kv_quant_write(kv, cache, pos, win, offset, rope_dim, n_valid)
 
 
 def kv_quant_read(cache: torch.Tensor, idx: torch.Tensor | None = None, D: int = 512, rope_dim: int = 64,
@@ -484,29 +342,7 @@ def kv_quant_read(cache: torch.Tensor, idx: torch.Tensor | None = None, D: int =
     row bytes]; idx [B, K] int32 (negative: a zero row; >= rows: clamped,
     ``status`` bit 1) or None for every row -> [B, K, D] bf16, or fp32 (the
     products of code and scale, not rounded) with ``dtype=torch.float32``."""
-    B = cache.shape[0]
-    _quant_cache(cache, B, D, rope_dim)
-    if dtype not in (BF16, F32):
-        raise ValueError(f"dtype must be bfloat16 or float32, got {dtype}")
-    K, ld = cache.shape[1], 0
-    if idx is not None:
-        _need(idx, "idx", I32)
-        if idx.dim() != 2 or idx.shape[0] != B or (idx.stride(1) != 1 and idx.shape[1] > 1):
-            raise ValueError(f"idx must be [{B}, K] with a unit stride in the last dim")
-        K = idx.shape[1]
-        ld = idx.stride(0) if B > 1 else K
-    stream = _launch_stream(cache, idx, out, status)
-    if out is None:
-        out = torch.empty((B, K, D), dtype=dtype, device=cache.device)
-    else:
-        _need(out, "out", dtype)
-        _contig(out, "out")
-        if out.shape != (B, K, D):
-            raise ValueError(f"out must be {(B, K, D)}, got {tuple(out.shape)}")
-    if B and K:
-        check(lib().dsa_kv_quant_read(cache.data_ptr(), cache.stride(0), cache.shape[1], _ptr(idx), ld, out.data_ptr(),
-                                      dtype == F32, B, K, D, rope_dim, _ptr(status), stream), "kv_quant_read")
-    return out
+    return _native().kv_quant_read(cache, idx, D, rope_dim, dtype, out, status)
 
 
 def kv_window_write(kv: torch.Tensor, kv_cache: torch.Tensor, pos: torch.Tensor, win: int,
@@ -1027,48 +863,7 @@ def sparse_attn_quant(q, cache, idx, sink, scale: float, out=None, lse=None, ws:
     [B,64,512] bf16; cache [>=B, rows, 608] uint8 (kv_quant_cache); idx
     [B,S,K] / [B,K] int32, negative = masked; sink [64] fp32.  Without ``ws``
     the scratch is allocated on the current stream for this call."""
-    _need(q, "q", BF16)
-    _contig(q, "q")
-    _need(idx, "idx", I32)
-    _need(sink, "sink", F32)
-    _contig(sink, "sink")
-    *lead, H, D = q.shape if q.dim() >= 2 else (0, 0)
-    if len(lead) not in (1, 2):
-        raise ValueError("q must be [B, S, H, D] or [B, H, D]")
-    if H != 64 or D != 512 or sink.numel() != H:
-        raise ValueError(f"sparse_attn_quant: built for 64 heads of 512 dims and as many sinks (got {H} of {D}, "
-                         f"{sink.numel()} sinks)")
-    B, S = lead[0], lead[1] if len(lead) == 2 else 1
-    _quant_cache(cache, B, D, 64)
-    *ilead, K = idx.shape if idx.dim() else (0,)
-    if ilead != lead and (S != 1 or ilead not in ([B], [B, 1])):
-        raise ValueError(f"idx must be [B, S, K] for q {tuple(q.shape)}, got {tuple(idx.shape)}")
-    ld_idx = _row_stride(idx, "idx") if K else 0
-    stream = _launch_stream(q, cache, idx, sink, out, lse, status)
-    if out is None:
-        out = torch.empty_like(q)
-    else:
-        _need(out, "out", BF16)
-        _contig(out, "out")
-        if out.shape != q.shape:
-            raise ValueError("out must have q's shape")
-    if lse is not None:
-        _need(lse, "lse", F32)
-        _contig(lse, "lse")
-        if lse.numel() != B * S * H:
-            raise ValueError(f"lse has {lse.numel()} elements, expected {B * S * H}")
-    if B == 0 or S == 0:
-        return out
-    need = _attn_ws[q.get_device(), B, S, K]
-    buf = None
-    if need:
-        buf = ws.get(need) if ws is not None else torch.empty(need, dtype=_U8, device=q.device)
-    check(lib().dsa_sparse_attn_quant(q.data_ptr(), cache.data_ptr(), cache.stride(0), cache.shape[1],
-                                      idx.data_ptr() if K else sink.data_ptr(), ld_idx, sink.data_ptr(),
-                                      out.data_ptr(), None if lse is None else lse.data_ptr(), B, S, H, D, K, scale,
-                                      None if buf is None else buf.data_ptr(), need,
-                                      None if status is None else status.data_ptr(), stream), "sparse_attn_quant")
-    return out
+    return _native().sparse_attn_quant(q, cache, idx, sink, scale, out, lse, ws, status)
 
 
 def sparse_attn_partial(q, kv, idx, scale: float, part_ml=None, part_o=None, ws: Workspace | None = None,
