@@ -42,7 +42,6 @@ struct WriteArgs {
   float inv_max;
 };
 
-// Sequences along y, groups of kRows tokens along x: a warp takes one group.
 // the two bf16 of a 32-bit word, divided by s, as e4m3 codes (neg_r2: -r twice)
 __device__ __forceinline__ uint32_t quotient_codes(uint32_t w, uint64_t neg_r2, uint64_t s2) {
   uint64_t nx, q, e;
@@ -62,6 +61,7 @@ __device__ __forceinline__ uint64_t twice(float v) {
 }
 __device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
 
+// Sequences along y, groups of kRows tokens along x: a warp takes one group.
 __global__ void __launch_bounds__(32 * kWarps) kv_quant_write_kernel(const WriteArgs a) {
   pdl_wait();
   pdl_launch_dependents();
@@ -83,14 +83,20 @@ __global__ void __launch_bounds__(32 * kWarps) kv_quant_write_kernel(const Write
         dst[u] = a.cache + b * a.bstride + (a.offset + uint32_t(pos + s0 + u) % uint32_t(a.win)) * a.rec;
       // the chunk count is not a multiple of 32 in general: whole warps take
       // part in the shuffles of a partly filled round
-      for (int c0 = 0; c0 < all_chunks; c0 += 32) {
-        const int c = c0 + lane;
-        uint4 raw[kRows];
+      uint4 raw[kRows], next[kRows];
+      auto fetch = [&](int c) {
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
-          raw[u] = make_uint4(0, 0, 0, 0);
-          if (c < all_chunks && s0 + u < n) raw[u] = __ldg(reinterpret_cast<const uint4*>(src + u * a.ld_s) + c);
+          next[u] = make_uint4(0, 0, 0, 0);
+          if (c < all_chunks && s0 + u < n) next[u] = __ldg(reinterpret_cast<const uint4*>(src + u * a.ld_s) + c);
         }
+      };
+      fetch(lane);
+      for (int c0 = 0; c0 < all_chunks; c0 += 32) {
+        const int c = c0 + lane;
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) raw[u] = next[u];
+        fetch(c + 32);  // the next round's while this one is worked on
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
           // the block's maximum as bf16: a NaN stays
