@@ -7,7 +7,7 @@
 // reciprocal r of the block's s (one a lane) by Markstein's correction:
 //   q = fl(x r), e = fl(q s - x) (exact in an FMA), fl(q - e r)
 // (in this sign a negative zero keeps its sign), two elements an instruction
-// (a division each: 13.9 us for the 20,000 rows below, against 11.1).
+// (a division each: 13.9 us for the 20,000 rows below, against 11.1 then).
 // |x| >= 2^-10 s wherever the code is not zero and 2^-23 < s < 2^120, so
 // nothing under- or overflows that the result shows.
 // Read: bf16(float(code) * s), the rotary dims as they are.
@@ -16,9 +16,10 @@
 // bf16 on one side, a 608-B record on the other at 448 + 64 dims).  Measured:
 // reading 132,000 selected records of 64 sequences 42.4 us, 5.36 TB/s (one row
 // a warp at a time and 64-bit divisions for its place: 53.1); writing the
-// 20,000 live rows of 8 padded sequences 11.3 us, about half of it two waves'
-// latency of n_valid, pos and the row one after the other; one row each of 64
-// sequences 2.4 us.
+// 20,000 live rows of 8 padded sequences 10.2 us (the two rounds of a row's
+// chunks fetched one after the other: 11.4; one or four rows a warp: 11.1,
+// 11.8), about half of it two waves' latency of n_valid, pos and the row one
+// after the other; one row each of 64 sequences 2.1 us.
 #include "kv_quant_dev.cuh"
 
 namespace dsa {

@@ -30,10 +30,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // (M, L, sum_p o_p e^{m_p-M}) without the sink.  One warp per (query row,
 // head, slice of DPL * 32 output dims): the split statistics are reduced
 // across lanes (any number of splits), then lane l combines DPL dims of
-// every split, eight splits' loads in flight at a time.  DPL = 16 covers the
-// 512 dims with one warp (many query rows); DPL = 4 spreads a row over 4x
-// more warps for the few-row case (a single long context), where the
-// combine would otherwise run on M * 8 CTAs.
+// every split.  DPL = 16 covers the 512 dims with one warp (many query
+// rows); DPL = 4 spreads a row over 4x more warps for the few-row case (a
+// single long context), where the combine would otherwise run on M * 8 CTAs.
 constexpr int kCombineWarps = 8;
 template <int DPL, bool kNormBF16>
 __global__ void __launch_bounds__(32 * kCombineWarps) lse_combine_kernel(
@@ -46,6 +45,31 @@ __global__ void __launch_bounds__(32 * kCombineWarps) lse_combine_kernel(
   pdl_launch_dependents();
   if (h >= H) return;
   auto ml = [&](int p, int j) { return part_ml[int64_t(p) * ml_ps + (int64_t(m) * H + h) * 2 + j]; };
+  const int d0 = blockIdx.z * (32 * DPL) + DPL * lane;
+  // U splits' partials in flight, the first ones fetched before the statistics
+  // are reduced (eight at a time after them and the last ones one by one: 15.5
+  // us for one row's attention over 17 splits and their combine, now
+  // 14.4; 37 rows of 4 splits 26.2 -> 23.9).  16 fp32 dims a lane take one: more
+  // registers cost warps (64 rows of 17 partials: eight 33.8 us, two 31.0, one
+  // 25.2).
+  constexpr int U = DPL == 4 ? (kNormBF16 ? 16 : 8) : (kNormBF16 ? 8 : 1);
+  using Vec = std::conditional_t<kNormBF16, uint2, float4>;  // 4 dims
+  Vec v[U][DPL / 4];
+  auto fetch = [&](int p0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (p0 + u < P) {
+        const int64_t off = int64_t(p0 + u) * o_ps + (int64_t(m) * H + h) * D + d0;
+        const Vec* src;
+        if constexpr (kNormBF16)
+          src = reinterpret_cast<const Vec*>(static_cast<const __nv_bfloat16*>(part_o) + off);
+        else
+          src = reinterpret_cast<const Vec*>(static_cast<const float*>(part_o) + off);
+#pragma unroll
+        for (int i = 0; i < DPL / 4; ++i) v[u][i] = __ldg(src + i);
+      }
+  };
+  fetch(0);
   float Mx = final_mode ? sink[h] : -INFINITY;
   for (int p0 = 0; p0 < P; p0 += 32) {
     const float mp = p0 + lane < P ? ml(p0 + lane, 0) : -INFINITY;
@@ -60,53 +84,43 @@ __global__ void __launch_bounds__(32 * kCombineWarps) lse_combine_kernel(
   }
   float L = warp_sum(lsum);
   if (final_mode && Mx != -INFINITY) L += expf(sink[h] - Mx);
-  const int d0 = blockIdx.z * (32 * DPL) + DPL * lane;
   float acc[DPL];
 #pragma unroll
   for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
   // Lane p of a group of 32 splits works out its weight, the loop takes it by a
-  // shuffle: only the partials' loads are left in it, eight splits in flight
-  // (a weight in every lane, four in flight: 17.1 us for one row's attention
-  // over 17 splits and their combine, now 15.5; the same sums in the same order).
-  for (int p0 = 0; p0 < P; p0 += 32) {
-    float wl = 0.f;
-    if (p0 + lane < P) {
-      const float mp = ml(p0 + lane, 0);
-      wl = (mp == -INFINITY) ? 0.f : expf(mp - Mx);
-      if constexpr (kNormBF16) wl *= ml(p0 + lane, 1);
+  // shuffle: only the partials' loads are left in it.
+  static_assert(32 % U == 0, "a group's weights cover whole batches");
+  float wl = 0.f;
+  for (int p0 = 0; p0 < P; p0 += U) {
+    if (p0 % 32 == 0) {
+      wl = 0.f;
+      if (p0 + lane < P) {
+        const float mp = ml(p0 + lane, 0);
+        wl = (mp == -INFINITY) ? 0.f : expf(mp - Mx);
+        if constexpr (kNormBF16) wl *= ml(p0 + lane, 1);
+      }
     }
-    const int n = min(32, P - p0);
-#pragma unroll 8
-    for (int q = 0; q < n; ++q) {
-      const float w = __shfl_sync(0xffffffffu, wl, q);
-      const int64_t off = int64_t(p0 + q) * o_ps + (int64_t(m) * H + h) * D + d0;
-      if constexpr (kNormBF16) {
-        // DPL bf16 values = DPL / 4 8-byte words
-        const uint2* src = reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(part_o) + off);
-        uint2 v[DPL / 4];
 #pragma unroll
-        for (int i = 0; i < DPL / 4; ++i) v[i] = __ldg(src + i);
+    for (int u = 0; u < U; ++u) {
+      if (p0 + u >= P) break;
+      const float w = __shfl_sync(0xffffffffu, wl, (p0 + u) & 31);
 #pragma unroll
-        for (int i = 0; i < DPL / 4; ++i) {
-          acc[4 * i + 0] = fmaf(w, __uint_as_float(v[i].x << 16), acc[4 * i + 0]);
-          acc[4 * i + 1] = fmaf(w, __uint_as_float(v[i].x & 0xffff0000u), acc[4 * i + 1]);
-          acc[4 * i + 2] = fmaf(w, __uint_as_float(v[i].y << 16), acc[4 * i + 2]);
-          acc[4 * i + 3] = fmaf(w, __uint_as_float(v[i].y & 0xffff0000u), acc[4 * i + 3]);
-        }
-      } else {
-        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(part_o) + off);
-        float4 v[DPL / 4];
-#pragma unroll
-        for (int i = 0; i < DPL / 4; ++i) v[i] = __ldg(src + i);
-#pragma unroll
-        for (int i = 0; i < DPL / 4; ++i) {
-          acc[4 * i + 0] = fmaf(w, v[i].x, acc[4 * i + 0]);
-          acc[4 * i + 1] = fmaf(w, v[i].y, acc[4 * i + 1]);
-          acc[4 * i + 2] = fmaf(w, v[i].z, acc[4 * i + 2]);
-          acc[4 * i + 3] = fmaf(w, v[i].w, acc[4 * i + 3]);
+      for (int i = 0; i < DPL / 4; ++i) {
+        const Vec x = v[u][i];
+        if constexpr (kNormBF16) {
+          acc[4 * i + 0] = fmaf(w, __uint_as_float(x.x << 16), acc[4 * i + 0]);
+          acc[4 * i + 1] = fmaf(w, __uint_as_float(x.x & 0xffff0000u), acc[4 * i + 1]);
+          acc[4 * i + 2] = fmaf(w, __uint_as_float(x.y << 16), acc[4 * i + 2]);
+          acc[4 * i + 3] = fmaf(w, __uint_as_float(x.y & 0xffff0000u), acc[4 * i + 3]);
+        } else {
+          acc[4 * i + 0] = fmaf(w, x.x, acc[4 * i + 0]);
+          acc[4 * i + 1] = fmaf(w, x.y, acc[4 * i + 1]);
+          acc[4 * i + 2] = fmaf(w, x.z, acc[4 * i + 2]);
+          acc[4 * i + 3] = fmaf(w, x.w, acc[4 * i + 3]);
         }
       }
     }
+    if (p0 + U < P) fetch(p0 + U);
   }
   if (final_mode) {
     const float inv = 1.f / L;
