@@ -291,3 +291,14 @@ def test_linear_captured_and_on_two_streams(cuda_dev):
         torch.cuda.synchronize()
         assert all(torch.equal(o, wt) for o, wt in zip(outs, want))
         assert all(torch.equal(e, want[2]) for e in eager)
+
+
+def test_workspace_of_another_device(cuda_dev):
+    from dsv4attn import ops
+    w = ops.pack_linear_weight_mxfp4(_x(256, 4096, BF, 1).to(cuda_dev))
+    x = _x(512, 4096, BF, 2).to(cuda_dev)
+    with pytest.raises(ValueError, match="workspace on cpu"):
+        ops.linear_mxfp4(x, w, ws=ops.Workspace("cpu"))
+    ws = ops.Workspace(cuda_dev)
+    assert torch.equal(ops.linear_mxfp4(x, w, ws=ws), ops.linear_mxfp4(x, w))
+    assert ws.nbytes > 16

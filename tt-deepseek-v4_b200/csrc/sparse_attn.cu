@@ -178,7 +178,9 @@ static SplitPlan plan_splits(int M, int K) {
   int tps = (ntiles + want - 1) / want;
   // at least two tiles per split: a CTA's fixed cost (Q load, TMEM set-up,
   // 128 KB partial out, its share of the combine) outweighs a second tile
-  // (few-row shapes: 1 row x 34 tiles 18.2 -> 15.8 us, 4 rows 21.5 -> 18.0 us)
+  // (few-row shapes: 1 row x 34 tiles 18.2 -> 15.8 us, 4 rows 21.5 -> 18.0 us;
+  // with the combine as it is now 1 row of records takes 13.9 us at one tile
+  // a split against 14.4, not taken: another split rounds otherwise)
   tps = std::max(tps, std::min(2, ntiles));
   tps = std::min(tps, idx_cap() / tile);  // the kernel stages <= kIdxCap indices
   return {(ntiles + tps - 1) / tps, tps};

@@ -111,7 +111,11 @@ Tensor empty_like_type(at::IntArrayRef shape, const Tensor& t, at::ScalarType dt
 
 // scratch: from the caller's Workspace, or of the current stream
 Tensor scratch(const py::object& ws, size_t bytes, const Tensor& like) {
-  if (!ws.is_none()) return py::cast<Tensor>(ws.attr("get")(bytes));
+  if (!ws.is_none()) {
+    Tensor buf = py::cast<Tensor>(ws.attr("get")(bytes));
+    if (buf.device() != like.device()) bad("workspace on ", buf.device(), ", tensors on ", like.device());
+    return buf;
+  }
   return empty_like_type({int64_t(bytes)}, like, at::kByte);
 }
 
