@@ -74,8 +74,8 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f for i in inc for f in ("-isystem", i)), TORCH_SRC, "-o", tmp, "-L" + OUT_DIR, "-l:libdsv4attn.so",
-           "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(tdir, "lib"), "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python",
-           "-lc10_cuda"]
+           "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(tdir, "lib"), "-lc10", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
+           "-ltorch_python", "-lc10_cuda"]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)

@@ -1,10 +1,11 @@
 // The low-bit operators over torch tensors: argument checks, allocation of
 // what the caller does not pass, the current stream, then the C ABI
 // (include/dsv4attn.h).  Compiled, because a decode step calls them with
-// kernels of 2-10 us: through ctypes a call took the host 12-19 us, here 2.7
-// (cache write) to 7.7 (projection of 64 tokens, two launches and two
+// kernels of 2-10 us: through ctypes a call took the host 12-19 us, here 2.8
+// (cache write) to 7.6 (projection of 64 tokens, two launches and two
 // allocations); a launch is ~2 of it.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -105,8 +106,11 @@ int32_t* status_of(const Opt& t) {
   return data<int32_t>(t);
 }
 
+// Past the dispatcher, 0.3-0.4 us a tensor less (a quantisation's three: 6.4 ->
+// 5.6 us a call).  What it leaves out besides, the deterministic mode's fill,
+// is not needed: every element is written.
 Tensor empty_like_type(at::IntArrayRef shape, const Tensor& t, at::ScalarType dtype) {
-  return at::empty(shape, t.options().dtype(dtype).requires_grad(false));
+  return at::detail::empty_cuda(shape, dtype, t.device(), std::nullopt);
 }
 
 // scratch: from the caller's Workspace, or of the current stream
