@@ -202,3 +202,12 @@ def test_a_missing_module_is_an_error(monkeypatch):
     monkeypatch.delattr("dsv4attn._torch_ops", raising=False)
     with pytest.raises(_lib.NativeLibraryError, match="build.py"):
         _lib.torch_ops()
+
+
+def test_a_ring_behind_the_cache_is_refused_at_any_offset():
+    """offset + win past 2^63 must not come round to a small number."""
+    from dsv4attn import _lib
+    f = _lib.lib().dsa_kv_quant_write
+    for offset in (2**63 - 8, 2**63 - 1, 2**62, 1):
+        _refused(f(16, 512, 512, 16, 608 * 8, 8, 16, None, 2, 0, 512, 64, 8, offset, None), "ring")
+    assert f(16, 512, 512, 16, 608 * 8, 8, 16, None, 2, 0, 512, 64, 8, 0, None) == _lib.DSA_OK

@@ -237,7 +237,7 @@ extern "C" int dsa_kv_quant_write(const void* kv, int64_t ld_b, int64_t ld_s, vo
   DSA_CHECK_ARG(kv && cache && pos, "kv_quant_write: null kv/cache/pos");
   const int rc = kvq::check_row("kv_quant_write", cache, cache_bstride, cache_rows, B, D, rope_dim);
   if (rc) return rc;
-  DSA_CHECK_ARG(S >= 0 && win > 0 && offset >= 0 && offset + win <= cache_rows,
+  DSA_CHECK_ARG(S >= 0 && win > 0 && offset >= 0 && win <= cache_rows && offset <= cache_rows - win,
                 "kv_quant_write: the ring's rows [offset, offset + win) must lie in the cache");
   DSA_CHECK_ARG(aligned(kv, 16) && ld_b % 8 == 0 && ld_s % 8 == 0,
                 "kv_quant_write: kv needs 16-byte alignment and strides that are multiples of 8 elements");
