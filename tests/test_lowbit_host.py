@@ -211,3 +211,19 @@ def test_a_ring_behind_the_cache_is_refused_at_any_offset():
     for offset in (2**63 - 8, 2**63 - 1, 2**62, 1):
         _refused(f(16, 512, 512, 16, 608 * 8, 8, 16, None, 2, 0, 512, 64, 8, offset, None), "ring")
     assert f(16, 512, 512, 16, 608 * 8, 8, 16, None, 2, 0, 512, 64, 8, 0, None) == _lib.DSA_OK
+
+
+def test_a_packed_weight_smaller_than_its_sizes_is_refused():
+    """The kernel streams ceil(N/128) x ceil(K/256) tiles of 17,408 bytes."""
+    from dsv4attn import ops
+    x = torch.zeros(2, 512, dtype=BF)
+    tiles = 2 * 2 * 17408                                  # N = 129, K = 512
+    bad = [(torch.zeros(tiles - 1, dtype=torch.uint8), 129, 512), (torch.zeros(tiles, dtype=torch.uint8), 257, 512),
+           (torch.zeros(tiles, dtype=torch.int8), 129, 512), (torch.zeros(2 * tiles, dtype=torch.uint8)[::2], 129, 512),
+           (torch.zeros(tiles, dtype=torch.uint8), 129, 500), (torch.zeros(tiles, dtype=torch.uint8), 0, 512),
+           (torch.zeros(tiles, dtype=torch.uint8), 2**32 + 129, 512)]
+    for packed, N, K in bad:
+        with pytest.raises(ValueError, match="packed"):
+            ops.linear_mxfp4(x, ops.MXFP4Weight(packed, N, K))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.linear_mxfp4(x, ops.MXFP4Weight(torch.zeros(tiles, dtype=torch.uint8), 129, 512))

@@ -168,6 +168,11 @@ py::tuple mxfp4_quant(const Tensor& x, const py::object& out_arg, Opt codes, Opt
 
 Tensor linear_mxfp4(const Tensor& x, const Tensor& packed, int64_t N, int64_t K, const Opt& out_arg, bool out_f32,
                     const py::object& ws, const Opt& status) {
+  // the product reads every tile that N and K name
+  const size_t tiles = N > 0 && N <= INT32_MAX && K > 0 && K <= INT32_MAX ? dsa_linear_mxfp4_packed_bytes(int(N), int(K)) : 0;
+  if (tiles == 0 || packed.scalar_type() != at::kByte || !packed.is_contiguous() || size_t(packed.numel()) < tiles)
+    bad("w's packed tensor must be the tiles of a [", N, ", ", K, "] weight (contiguous uint8, ", tiles,
+        " bytes), got ", dtype_name(packed.scalar_type()), " ", packed.sizes());
   need(x, "x");
   const int type = x_type(x);
   if (x.dim() != 2 || x.size(1) != K || x.stride(1) != 1)
