@@ -542,7 +542,7 @@ size_t dsa_sparse_attn_workspace_size(int B, int S, int H, int D, int K);
  * q [B*S, H, D] bf16; kv bf16 rows of D with batch stride kv_bstride and
  * kv_rows rows per batch (indices >= kv_rows are an error the kernel
  * clamps and reports through `status`); idx [B*S, K] int32 (row stride
- * ld_idx); sink [H] fp32; out [B*S, H, D] bf16.  lse (may be NULL):
+ * ld_idx; K at most 2^31 - 4609); sink [H] fp32; out [B*S, H, D] bf16.  lse (may be NULL):
  * [B*S, H] fp32 natural-log partition sum including the sink.
  * workspace: >= dsa_sparse_attn_workspace_size() bytes (may be NULL when
  * that is 0).  status (may be NULL): device int32, set non-zero if any

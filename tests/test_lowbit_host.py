@@ -227,3 +227,17 @@ def test_a_packed_weight_smaller_than_its_sizes_is_refused():
             ops.linear_mxfp4(x, ops.MXFP4Weight(packed, N, K))
     with pytest.raises(ValueError, match="CUDA"):
         ops.linear_mxfp4(x, ops.MXFP4Weight(torch.zeros(tiles, dtype=torch.uint8), 129, 512))
+
+
+def test_attention_refuses_an_index_list_whose_tiles_wrap():
+    """K + 63 must stay below 2^31: a wrapped tile count attended the first 64
+    entries only.  (A list this long is 8 GB of indices for one query row.)"""
+    from dsv4attn import _lib
+    L = _lib.lib()
+    for K in (2**31 - 1, 2**31 - 64, 2**31 - 4096):
+        assert L.dsa_sparse_attn_workspace_size(1, 1, 64, 512, K) == 0
+        _refused(L.dsa_sparse_attn_quant(16, 16, 608 * 8, 8, 16, K, 16, 16, None, 1, 1, 64, 512, K, 1.0, None, 0, None,
+                                         None), "K")
+        _refused(L.dsa_sparse_attn(16, 16, 512 * 8, 8, 16, K, 16, 16, None, 1, 1, 64, 512, K, 1.0, None, 0, None, None),
+                 "K")
+    assert L.dsa_sparse_attn_workspace_size(1, 1, 64, 512, 2**31 - 8192) > 2**31

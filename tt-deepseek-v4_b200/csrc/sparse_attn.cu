@@ -202,12 +202,15 @@ static void ensure_attr() {
   }
 }
 
+// index rows whose tile counts and split ends stay below 2^31
+constexpr int kMaxK = INT32_MAX - 2 * satc::kIdxCap;
+
 // quant: kv holds records of the FP8 latent cache and kv_bstride is in bytes
 static int check_common(const void* q, const void* kv, int64_t kv_bstride, int64_t kv_rows, const int32_t* idx,
                         int64_t ld_idx, int B, int S, int H, int D, int K, bool quant) {
   DSA_CHECK_ARG(q && kv && idx, "sparse_attn: null q/kv/idx");
   DSA_CHECK_ARG(H == kSaH && D == kSaD, "sparse_attn: built for H=64, D=512 (got H=%d D=%d)", H, D);
-  DSA_CHECK_ARG(B >= 0 && S >= 1 && K >= 0 && kv_rows > 0, "sparse_attn: bad B/S/K/kv_rows");
+  DSA_CHECK_ARG(B >= 0 && S >= 1 && K >= 0 && K <= kMaxK && kv_rows > 0, "sparse_attn: bad B/S/K/kv_rows");
   DSA_CHECK_ARG(int64_t(B) * S <= INT32_MAX / kSaH, "sparse_attn: B*S = %lld query rows is too many",
                 (long long)B * S);
   if (quant) {
@@ -230,8 +233,8 @@ using namespace dsa;
 extern "C" size_t dsa_sparse_attn_workspace_size(int B, int S, int H, int D, int K) {
   (void)H;
   (void)D;
-  // shapes the attention rejects (B*S beyond its row limit) need no workspace
-  if (B < 0 || S < 1 || int64_t(B) * S > INT32_MAX / kSaH) return 0;
+  // shapes the attention rejects (B*S or K beyond its limits) need no workspace
+  if (B < 0 || S < 1 || int64_t(B) * S > INT32_MAX / kSaH || K > kMaxK) return 0;
   const int M = B * S;
   return ws_bytes_for(plan_splits(M, K), M);
 }
