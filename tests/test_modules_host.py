@@ -66,3 +66,50 @@ def test_head_norm_rope_oracle_identities():
     n = ref.head_norm_rope(x, 2, 128, norm=True, weight=1.0)
     rms = n.float().view(3, 2, 128).pow(2).mean(-1).sqrt()
     assert torch.allclose(rms, torch.ones_like(rms), atol=2e-2)
+
+
+def _fp4(lin):
+    """The same Linear as MXFP4 codes of zeros with unit scales."""
+    n, k = lin.weight.shape
+    lin.weight = torch.zeros(n, k // 2, dtype=torch.int8)
+    lin.scale = torch.full((n, k // 32), 127, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+
+
+@pytest.mark.parametrize("kind", ["indexer", "twins", "compressor", "window"])
+@pytest.mark.parametrize("name", ["wq_a", "wq_b", "wkv", "wo_a", "wo_b"])
+def test_device_attention_refuses_mxfp4_weights(monkeypatch, kind, name):
+    """Every kind of layer refuses a 4-bit projection weight before anything is
+    packed: its product would quantise the activations too."""
+    from types import SimpleNamespace
+
+    from dsv4attn import modules as M
+    monkeypatch.setattr(M, "_device_of", lambda mesh: torch.device("cpu"))
+    attn, _, _ = make_block(seed=1, max_seq_len=64)
+    if kind == "twins":
+        attn._device_compressor = attn._device_indexer = SimpleNamespace()
+    if kind in ("compressor", "window"):
+        attn.indexer = None
+    if kind == "window":
+        attn.compress_ratio, attn.compressor = 0, None
+    _fp4(getattr(attn, name))
+    with pytest.raises(ValueError, match=f"{name}.*MXFP4"):
+        M.DeviceAttention(torch.device("cpu"), attn, sparse_attn_dev=SimpleNamespace())
+
+
+@pytest.mark.parametrize("path", ["compressor.wkv", "compressor.wgate", "indexer.wq_b", "indexer.weights_proj",
+                                  "indexer.compressor.wkv", "indexer.compressor.wgate"])
+def test_device_attention_refuses_mxfp4_weights_of_its_parts(monkeypatch, path):
+    from types import SimpleNamespace
+
+    from dsv4attn import modules as M
+    monkeypatch.setattr(M, "_device_of", lambda mesh: torch.device("cpu"))
+    attn, _, _ = make_block(seed=1, max_seq_len=64)
+    part = attn
+    for step in path.split("."):
+        part = getattr(part, step)
+    _fp4(part)
+    with pytest.raises(ValueError, match="MXFP4"):
+        M.DeviceAttention(torch.device("cpu"), attn, sparse_attn_dev=SimpleNamespace())
+    if path.startswith("indexer.w"):
+        with pytest.raises(ValueError, match="MXFP4"):
+            M.DeviceIndexer(torch.device("cpu"), attn.indexer, SimpleNamespace())

@@ -97,6 +97,14 @@ def mxfp4_parts(w):
     return t.detach().view(torch.uint8), scale.detach().view(torch.uint8)
 
 
+def _refuse_mxfp4(**weights):
+    """The decode block keeps bf16 activations, and the product over a 4-bit
+    weight quantises them (ops.linear_mxfp4)."""
+    for name, w in weights.items():
+        if w is not None and mxfp4_parts(w) is not None:
+            raise ValueError(f"{name}: MXFP4 weights are not taken here, expand them to bf16")
+
+
 def _gamma_of(norm, fallback=None) -> torch.Tensor:
     for name in ("_cpu_gamma", "gamma", "weight"):
         g = getattr(norm, name, None) if norm is not None else None
@@ -451,6 +459,8 @@ class DeviceIndexer(torch.nn.Module):
         self.compress_ratio = int(indexer.compress_ratio)
         self.softmax_scale = float(indexer.softmax_scale)
         self.index_topk = int(indexer.index_topk)
+        _refuse_mxfp4(wq_b=indexer.wq_b if wq_b_dev is None else None,
+                      weights_proj=indexer.weights_proj if weights_proj_dev is None else None)
         if wq_b_dev is None:
             wq_b_dev = DeviceLinear(self.device, indexer.wq_b)
         if weights_proj_dev is None:
@@ -522,6 +532,16 @@ class DeviceAttention(torch.nn.Module):
         super().__init__()
         dev = self.device = _device_of(mesh)
         self.attn = attn
+        _refuse_mxfp4(wq_a=attn.wq_a, wq_b=attn.wq_b, wkv=attn.wkv, wo_b=attn.wo_b,
+                      wo_a=wo_a_cpu_weight if wo_a_cpu_weight is not None else attn.wo_a)
+        if attn.compress_ratio:
+            comp = attn.compressor if getattr(attn, "_device_compressor", None) is None else None
+            ind = getattr(attn, "indexer", None) if getattr(attn, "_device_indexer", None) is None else None
+            if comp is not None:
+                _refuse_mxfp4(compressor_wkv=comp.wkv, compressor_wgate=comp.wgate)
+            if ind is not None:
+                _refuse_mxfp4(indexer_wq_b=ind.wq_b, indexer_weights_proj=ind.weights_proj,
+                              indexer_compressor_wkv=ind.compressor.wkv, indexer_compressor_wgate=ind.compressor.wgate)
         self.dim = int(attn.dim)
         self.n_heads = int(attn.n_local_heads)
         self.n_local_heads = self.n_heads
