@@ -241,3 +241,13 @@ def test_attention_refuses_an_index_list_whose_tiles_wrap():
         _refused(L.dsa_sparse_attn(16, 16, 512 * 8, 8, 16, K, 16, 16, None, 1, 1, 64, 512, K, 1.0, None, 0, None, None),
                  "K")
     assert L.dsa_sparse_attn_workspace_size(1, 1, 64, 512, 2**31 - 8192) > 2**31
+
+
+def test_the_package_imports_on_a_torch_without_cuda():
+    import os
+    import subprocess
+    import sys
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tt-deepseek-v4_b200")
+    code = ("import sys, torch; del torch._C._cuda_getCurrentRawStream; sys.path.insert(0, sys.argv[1]); "
+            "import dsv4attn; from dsv4attn import modules, ops")
+    subprocess.run([sys.executable, "-c", code, pkg], check=True, timeout=300)

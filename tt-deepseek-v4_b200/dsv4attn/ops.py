@@ -20,14 +20,11 @@ I32 = torch.int32
 F32 = torch.float32
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
 def _stream(t: torch.Tensor):
     """cudaStream_t of the current stream on t's device (the handle of
     torch.cuda.current_stream without building the Stream object: 0.1
     against 2 us a call)."""
-    return _raw_stream(t.get_device())
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _need(t: torch.Tensor, name: str, dtype=None, cuda=True):
