@@ -251,3 +251,33 @@ def test_the_package_imports_on_a_torch_without_cuda():
     code = ("import sys, torch; del torch._C._cuda_getCurrentRawStream; sys.path.insert(0, sys.argv[1]); "
             "import dsv4attn; from dsv4attn import modules, ops")
     subprocess.run([sys.executable, "-c", code, pkg], check=True, timeout=300)
+
+
+def test_the_module_is_rebuilt_for_another_torch_or_python(monkeypatch, tmp_path):
+    """The compiled module links torch's C++ internals, so file times alone do
+    not say that it is up to date."""
+    from types import SimpleNamespace
+
+    import build
+    ran = []
+
+    def run(cmd, check):
+        ran.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+    monkeypatch.setattr(build, "TORCH_LIB", str(tmp_path / "_torch_ops.so"))
+    monkeypatch.setattr(build, "OBJ_DIR", str(tmp_path / "obj"))
+    monkeypatch.setattr(build, "subprocess", SimpleNamespace(run=run))
+    assert build.build_torch_ops() == build.TORCH_LIB and len(ran) == 1
+    build.build_torch_ops()
+    assert len(ran) == 1
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    build.build_torch_ops()
+    build.build_torch_ops()
+    assert len(ran) == 2
+    monkeypatch.setattr(torch._C, "_GLIBCXX_USE_CXX11_ABI", not torch._C._GLIBCXX_USE_CXX11_ABI)
+    build.build_torch_ops()
+    assert len(ran) == 3
+    monkeypatch.setattr(build.sysconfig, "get_config_var", lambda name: "another python")
+    build.build_torch_ops()
+    build.build_torch_ops()
+    assert len(ran) == 4

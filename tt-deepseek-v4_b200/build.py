@@ -8,7 +8,8 @@ CUDA runtime, so the process that loads it through ctypes shares one
 runtime (and one primary context) with PyTorch.  ``csrc/torch_ops.cpp`` (the
 low-bit operators over torch tensors) becomes ``dsv4attn/_torch_ops.so``, a
 Python module linked against that library and torch.  Objects are rebuilt
-only when a source or header is newer than the library.
+only when a source or header is newer than the library, the module also when
+torch or Python is not the one it was built with.
 """
 
 from __future__ import annotations
@@ -59,10 +60,16 @@ def needs_build() -> bool:
 
 def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
     """The Python module over torch tensors (needs the library built)."""
-    deps = [TORCH_SRC, __file__] + glob.glob(os.path.join(INCLUDE, "*.h"))
-    if not force and os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) > max(map(os.path.getmtime, deps)):
-        return TORCH_LIB
     import torch
+    deps = [TORCH_SRC, __file__] + glob.glob(os.path.join(INCLUDE, "*.h"))
+    # it links torch's C++ internals and the interpreter's
+    made_with = f"torch {torch.__version__} abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)} {sysconfig.get_config_var('SOABI')}"
+    key = os.path.join(OBJ_DIR, "_torch_ops.key")
+    if not force and os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) > max(map(os.path.getmtime, deps)) \
+            and os.path.exists(key):
+        with open(key) as f:
+            if f.read() == made_with:
+                return TORCH_LIB
     tdir = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(find_nvcc())))
     inc = [os.path.join(tdir, "include"), os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
@@ -80,6 +87,9 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, TORCH_LIB)
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with open(key, "w") as f:
+        f.write(made_with)
     return TORCH_LIB
 
 
