@@ -130,9 +130,9 @@ int dsa_linear_mxfp4_pack(const uint8_t* codes, const uint8_t* scales, int N, in
  * infinity takes code 255 (NaN) and zero elements.
  * codes [M, K/2]: two elements a byte, the even one in the low half; scales
  * [M, K/32]; both contiguous.  out [M, K] of x's type, row stride ld_out (may
- * be NULL; may be x): the values the codes stand for, NaN in a block of code
- * 255.  K a multiple of 32; x and out 16-byte aligned, their row strides
- * multiples of 16 bytes; codes 4-byte aligned.
+ * be NULL; may be x itself, with ld_x; no other overlap): the values the codes
+ * stand for, NaN in a block of code 255.  K a multiple of 32; x and out 16-byte
+ * aligned, their row strides multiples of 16 bytes; codes 4-byte aligned.
  * The 4-bit counterpart of dsa_act_quant_block; the reference reads such
  * weights (inference.py:283-327) and expands them. */
 enum { DSA_BF16 = 0, DSA_FP16 = 1, DSA_FP32 = 2 };

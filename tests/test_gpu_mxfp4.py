@@ -80,6 +80,23 @@ def test_quant_strides_in_place_and_leading_dims(cuda_dev):
     assert empty[0].shape == (0, 64) and empty[2].shape == (0, 32)
 
 
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("M,K", [(1, 32), (65, 96), (4000, 4096)])
+def test_quant_in_place_is_quant(cuda_dev, dtype, M, K):
+    """out = x, whole rows and a column slice, gives what a separate out does."""
+    from dsv4attn import ops
+    x = _x(M, K, dtype, 3 * M + K).to(cuda_dev)
+    out, scales, codes = ops.mxfp4_quant(x, out=True)
+    wide = torch.full((M, K + 64), 7.0, dtype=dtype, device=cuda_dev)
+    wide[:, 32:32 + K] = x
+    for buf in (x.clone(), wide[:, 32:32 + K]):
+        got, s, c = ops.mxfp4_quant(buf, out=buf)
+        torch.cuda.synchronize()
+        assert got.data_ptr() == buf.data_ptr()
+        assert torch.equal(buf, out) and torch.equal(s, scales) and torch.equal(c, codes)
+    assert bool((wide[:, :32] == 7).all()) and bool((wide[:, 32 + K:] == 7).all())
+
+
 def test_quant_refusals(cuda_dev):
     from dsv4attn import ops
     d = cuda_dev

@@ -35,11 +35,22 @@ struct Shape {
   static constexpr int kUnroll = 2 / H;             // blocks a lane has in flight
 };
 
+// Eight elements by plain loads: out may be x, so x is neither __restrict__ nor
+// read through the non-coherent path.  A block's loads all precede its stores
+// (its maximum is exchanged between them), and no other block's elements lie
+// in its place.
+template <typename T>
+__device__ __forceinline__ Vec8<T> load8_plain(const T* p) {
+  Vec8<T> r;
+#pragma unroll
+  for (int i = 0; i < int(sizeof(T) / 2); ++i) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  return r;
+}
+
 // Blocks [0, blocks) in row order; the codes and scales are contiguous, x and
 // out have row strides.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) mxfp4_quant_kernel(const T* __restrict__ x, int64_t ld_x,
-                                                               T* __restrict__ out, int64_t ld_out,
+__global__ void __launch_bounds__(kThreads) mxfp4_quant_kernel(const T* x, int64_t ld_x, T* out, int64_t ld_out,
                                                                uint32_t* __restrict__ codes,
                                                                uint8_t* __restrict__ scales, int64_t blocks,
                                                                int row_blocks) {
@@ -64,7 +75,7 @@ __global__ void __launch_bounds__(kThreads) mxfp4_quant_kernel(const T* __restri
       }
 #pragma unroll
       for (int h = 0; h < S::H; ++h)
-        v[u][h] = at < blocks ? load8(x + row[u] * ld_x + col[u] + (h * S::kLanes + part) * kVec) : zero8<T>();
+        v[u][h] = at < blocks ? load8_plain(x + row[u] * ld_x + col[u] + (h * S::kLanes + part) * kVec) : zero8<T>();
     }
 #pragma unroll
     for (int u = 0; u < S::kUnroll; ++u) {
