@@ -448,3 +448,27 @@ def test_refusals_of_sizes_and_types_that_do_not_fit(cuda_dev):
     with pytest.raises(TypeError, match="out"):
         ops.mxfp4_quant(kv, out=False)
     assert not cache.any()
+
+
+def test_strides_that_nothing_steps_by(cuda_dev):
+    """One token, one sequence: the strides of those dims are not looked at."""
+    from dsv4attn import ops
+    d = cuda_dev
+    flat = _kv(1, 2, 512, seed=31).to(d).view(-1)
+    cache = torch.zeros(2, 4, 608, dtype=U8, device=d)
+    pos = torch.zeros(2, dtype=I32, device=d)
+    ops.kv_quant_write(flat.as_strided((2, 1, 512), (512, 3, 1)), cache, pos, 4)
+    want = torch.zeros_like(cache)
+    ops.kv_quant_write(flat.view(2, 512), want, pos, 4)
+    torch.cuda.synchronize()
+    assert torch.equal(cache, want) and bool(want.any())
+    one = want[1].clone().view(-1).as_strided((1, 4, 608), (5, 608, 1))
+    ops.kv_quant_write(flat.as_strided((1, 1, 512), (5, 3, 1)), one, pos[:1], 4, offset=0)
+    idx = torch.tensor([[0, 1, -1]], dtype=I32, device=d)
+    q = torch.randn(1, 64, 512, generator=torch.Generator().manual_seed(1)).to(BF).to(d)
+    sink = torch.zeros(64, device=d)
+    torch.cuda.synchronize()
+    assert torch.equal(one[0], want[0])
+    assert torch.equal(ops.kv_quant_read(one, idx), ops.kv_quant_read(want[:1], idx))
+    assert torch.equal(ops.sparse_attn_quant(q, one, idx, sink, SCALE),
+                       ops.sparse_attn_quant(q, want[:1], idx, sink, SCALE))

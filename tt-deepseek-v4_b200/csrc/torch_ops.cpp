@@ -229,6 +229,11 @@ void quant_cache(const Tensor& cache, int64_t B, int64_t D, int64_t rope_dim) {
         cache.sizes());
 }
 
+// bytes between sequences; of one sequence nothing steps by it
+int64_t cache_stride(const Tensor& cache, int64_t B) {
+  return B > 1 ? cache.stride(0) : cache.size(1) * cache.size(2);
+}
+
 void per_sequence(const Tensor& t, const char* name, int64_t B) {
   need(t, name, at::kInt);
   contig(t, name);
@@ -242,7 +247,7 @@ void kv_quant_write(const Tensor& kv_arg, const Tensor& cache, const Tensor& pos
   if ((d != 2 && d != 3) || kv_arg.stride(-1) != 1)
     bad("kv must be [B, S, D] or [B, D] with a unit stride in the last dim");
   const int64_t B = kv_arg.size(0), S = d == 3 ? kv_arg.size(1) : 1, D = kv_arg.size(-1);
-  const int64_t ld_b = kv_arg.stride(0), ld_s = d == 3 ? kv_arg.stride(1) : 0;
+  const int64_t ld_b = B > 1 ? kv_arg.stride(0) : 0, ld_s = S > 1 ? kv_arg.stride(1) : 0;
   quant_cache(cache, B, D, rope_dim);
   per_sequence(pos, "pos", B);
   if (n_valid) per_sequence(*n_valid, "n_valid", B);
@@ -250,7 +255,7 @@ void kv_quant_write(const Tensor& kv_arg, const Tensor& cache, const Tensor& pos
   if (B > INT32_MAX || S > INT32_MAX || win != int32_t(win)) bad("kv_quant_write: B, S or win is too large");
   if (B && S)
     call("kv_quant_write", [&] {
-      return dsa_kv_quant_write(kv_arg.data_ptr(), ld_b, ld_s, cache.data_ptr(), cache.stride(0), cache.size(1),
+      return dsa_kv_quant_write(kv_arg.data_ptr(), ld_b, ld_s, cache.data_ptr(), cache_stride(cache, B), cache.size(1),
                                 static_cast<const int32_t*>(pos.data_ptr()), data<const int32_t>(n_valid), int(B),
                                 int(S), int(D), int(rope_dim), int(win), offset, stream);
     });
@@ -285,7 +290,7 @@ Tensor kv_quant_read(const Tensor& cache, const Opt& idx, int64_t D, int64_t rop
   if (B > INT32_MAX) bad("kv_quant_read: B is too large");
   if (B && K)
     call("kv_quant_read", [&] {
-      return dsa_kv_quant_read(cache.data_ptr(), cache.stride(0), cache.size(1), data<const int32_t>(idx), ld,
+      return dsa_kv_quant_read(cache.data_ptr(), cache_stride(cache, B), cache.size(1), data<const int32_t>(idx), ld,
                                out.data_ptr(), dtype == at::kFloat, int(B), K, int(D), int(rope_dim), st, stream);
     });
   return out;
@@ -333,7 +338,7 @@ Tensor sparse_attn_quant(const Tensor& q, const Tensor& cache, const Tensor& idx
   Tensor buf;
   if (bytes) buf = scratch(ws, bytes, q);
   call("sparse_attn_quant", [&] {
-    return dsa_sparse_attn_quant(q.data_ptr(), cache.data_ptr(), cache.stride(0), cache.size(1),
+    return dsa_sparse_attn_quant(q.data_ptr(), cache.data_ptr(), cache_stride(cache, B), cache.size(1),
                                  static_cast<const int32_t*>(K ? idx.data_ptr() : sink.data_ptr()), ld_idx,
                                  static_cast<const float*>(sink.data_ptr()), out.data_ptr(), data<float>(lse), int(B),
                                  int(S), int(H), int(D), int(K), float(scale), bytes ? buf.data_ptr() : nullptr, bytes,
