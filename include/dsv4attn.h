@@ -101,7 +101,8 @@ int dsa_linear_pack(const void* w, int N, int K, int G, void* packed, size_t pac
  * bytes (the current device's; 0, and NULL will do, where the product
  * quantises X itself: a few tokens), 16-byte aligned, for X's codes and
  * scales; calls that can overlap need their own.  status (may be NULL): bit 2 when a
- * bounded wait ran out.
+ * bounded wait ran out; the rest of the call's waits then end early and Y is
+ * incomplete.
  * The 4-bit counterpart of dsa_linear; the reference expands such weights
  * (inference.py:283-327). */
 int dsa_linear_mxfp4(const void* x, int x_type, int64_t ld_x, const void* w_packed, void* y, int64_t ld_y, int B,

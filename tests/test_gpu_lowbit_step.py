@@ -126,3 +126,20 @@ def test_device_linear_with_mxfp4_weights(cuda_dev):
     with pytest.raises(ValueError, match="dtype"):
         M.DeviceLinear(cuda_dev, torch.zeros(32, 32, dtype=torch.int8))   # no scale: not MXFP4
     assert isinstance(lin.weight, ops.MXFP4Weight)
+
+
+def test_device_linear_mxfp4_has_a_status_word(cuda_dev, monkeypatch):
+    """A call that brings no status word still reports into one."""
+    from dsv4attn import modules as M
+    from dsv4attn import ops
+    seen = []
+    real = ops.linear_mxfp4
+    monkeypatch.setattr(ops, "linear_mxfp4", lambda *a, **k: (seen.append(k["status"]), real(*a, **k))[1])
+    a, b = _Fp4Linear(96, 256, 4), _Fp4Linear(160, 256, 5)
+    x = torch.randn(3, 256, generator=torch.Generator().manual_seed(1)).to(BF).to(cuda_dev)
+    own = torch.zeros(1, dtype=I32, device=cuda_dev)
+    for lin in (M.DeviceLinear(cuda_dev, a), M.DeviceLinear.fused(cuda_dev, [a, b])):
+        lin(x)
+        lin(x, status=own)
+        assert seen[-2] is lin.status and seen[-1] is own
+        ops.raise_for_status(lin.status, "linear_mxfp4")

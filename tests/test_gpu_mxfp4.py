@@ -319,3 +319,43 @@ def test_workspace_of_another_device(cuda_dev):
     ws = ops.Workspace(cuda_dev)
     assert torch.equal(ops.linear_mxfp4(x, w, ws=ws), ops.linear_mxfp4(x, w))
     assert ws.nbytes > 16
+
+
+@pytest.mark.parametrize("B,N,K", [(1024, 9600, 65536), (8, 128, 1 << 21)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_waits_that_run_out_end_the_call_once(cuda_dev, B, N, K, f32):
+    """A wait limit far below the sums' time, whole items and items split over a
+    cluster: the first wait to run out ends the others of its CTA, nothing wrong
+    is stored, the status says so, and the next call is right."""
+    import time
+
+    from dsv4attn import ops
+    g = torch.Generator(device=cuda_dev).manual_seed(B)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=U8, device=cuda_dev)
+    w = ops.pack_linear_weight_mxfp4(codes, torch.full((N, K // 32), 127, dtype=U8, device=cuda_dev))
+    del codes
+    x = torch.randn(B, K, generator=g, device=cuda_dev).to(BF)
+    want = ops.linear_mxfp4(x, w, out_f32=f32)
+    for width in (N, N + 1):                                # stored by tiles, and by elements
+        out = torch.full((B, width), 12345.0, dtype=want.dtype, device=cuda_dev)
+        blank = out[0, 0].clone()
+        status = torch.zeros(1, dtype=torch.int32, device=cuda_dev)
+        torch.cuda.synchronize()
+        prev = ops.set_wait_limit(1)
+        try:
+            t0 = time.time()
+            ops.linear_mxfp4(x, w, out=out, out_f32=f32, status=status)
+            torch.cuda.synchronize()
+            dt = time.time() - t0
+        finally:
+            ops.set_wait_limit(prev)
+        assert dt < 0.5, f"{dt:.3f} s"
+        with pytest.raises(TimeoutError):
+            ops.raise_for_status(status, "linear_mxfp4")
+        y = out[:, :N]
+        fine = (y == want) | (y == blank) | (y.isnan() if N == 128 else torch.zeros_like(y, dtype=torch.bool))
+        assert bool(fine.all()) and not torch.equal(y, want)
+        status.zero_()
+        again = ops.linear_mxfp4(x, w, out_f32=f32, status=status)
+        torch.cuda.synchronize()
+        assert torch.equal(again, want) and int(status) == 0

@@ -73,17 +73,18 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t par
       : "memory");
   return ok != 0;
 }
-// bounded, like tc::mbar_wait: a lost arrival ends in an error status
-__device__ __forceinline__ void mbar_wait_cluster(uint32_t bar, uint32_t parity, int32_t* status,
+// bounded, like tc::mbar_wait: a lost arrival ends in an error status (false)
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, int32_t* status,
                                                   long long limit) {
-  if (mbar_try_wait_cluster(bar, parity)) return;
+  if (mbar_try_wait_cluster(bar, parity)) return true;
   const long long t0 = clock64();
   while (!mbar_try_wait_cluster(bar, parity)) {
     if (clock64() - t0 > limit) {
       if (status) atomicOr(status, 2);
-      return;
+      return false;
     }
   }
+  return true;
 }
 
 }  // namespace lin

@@ -46,6 +46,13 @@
 // each CTA writes its partial [Bt][128] there, copies each owner's rows to it
 // through distributed shared memory, and the owner sums the C partials in rank
 // order: the same sum on every run.
+//
+// Every wait is bounded.  One that runs out sets a status bit and its CTA's
+// abort flag, at which the CTA's other waits return unless their phase is over:
+// its roles issue and store nothing more, what is in flight lands, and the CTA
+// leaves through the same barriers as ever.  Its tiles stay unwritten; a split
+// item's other owners get NaN from it.  (0-3 % of the times below: 64 x 32768 x 1024
+// 7.4 -> 7.7 us, 1024 x 4096 x 8192 27.8 -> 28.0.)
 #include "cluster.cuh"
 #include "common.cuh"
 #include "mxfp4_dev.cuh"
@@ -71,7 +78,7 @@ constexpr int kMaxStages = 8;
 constexpr int kMaxSplit = 16;
 constexpr int THREADS = 224;
 constexpr int kSmemBytes = 232448;
-constexpr int kAuxBytes = 256;
+constexpr int kAuxBytes = 512;
 constexpr int kFuseUnits = 48;                  // (token, k-block) units of X a CTA quantises itself, at most
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColSf = 2 * kMaxBt;         // scales of each stage: 8 columns of W, 8 a group of X
@@ -105,7 +112,10 @@ struct Aux {
   uint64_t acc_empty[2];
   uint64_t ready;
   uint64_t x_full;
+  uint64_t drained;    // gave up: the loads have landed, both issuers' work is done
   uint32_t tmem_base;
+  int abort;
+  int issued;          // stages whose loads were requested
 };
 static_assert(sizeof(Aux) <= kAuxBytes, "aux block");
 
@@ -114,6 +124,50 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
                    reinterpret_cast<uint64_t>(map)),
                "r"(src), "r"(x), "r"(y)
                : "memory");
+}
+
+// A phase's end, or false once the CTA has given up.  The loop lies inline only
+// in the fused kernel, whose few waits mostly begin before their phase's end
+// (inline / called: 8 x 1024 x 4096 5.47 / 5.60 us); inline everywhere, a
+// k-block of the ring takes 20 cycles more (1024 x 4096 x 8192: 28.8 / 27.9).
+__device__ __forceinline__ bool wait_loop(uint32_t bar, uint32_t parity, volatile int* abort, int32_t* status,
+                                          long long limit) {
+  const long long t0 = clock64();
+  for (;;) {
+    if (tc::mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+    if (clock64() - t0 > limit) {
+      if (status) atomicOr(status, 2);
+      *abort = 1;
+      return false;
+    }
+  }
+}
+__device__ __noinline__ bool wait_called(uint32_t bar, uint32_t parity, volatile int* abort, int32_t* status,
+                                         long long limit) {
+  return wait_loop(bar, parity, abort, status, limit);
+}
+
+// Warps 0, 1 and 6 of a CTA that gave up, once its roles have ended: `drained`
+// completes when its loads have landed and its tensor core work is done.  (A
+// limit of its own: the caller's may be too short for any of it.)
+__device__ __noinline__ void drain(Aux* aux, int n_stages, int32_t* status) {
+  if (threadIdx.x == 0) {
+    const int n = aux->issued;
+    for (int i = max(0, n - n_stages); i < n; ++i)
+      tc::mbar_wait(smem_u32(&aux->full[i % n_stages]), (i / n_stages) & 1, status, 2);
+    tc::mbar_arrive(smem_u32(&aux->drained));
+  } else if (threadIdx.x >= 32 && tc::elect_one()) {
+    tc::mma_commit(smem_u32(&aux->drained));
+  }
+  __syncwarp();
+  tc::mbar_wait(smem_u32(&aux->drained), 0, status, 2);
+}
+
+// The partial of a thread whose sums never came, once nothing else writes there
+__device__ __noinline__ void poison(float* column, int rows, const uint64_t* drained, int32_t* status) {
+  tc::mbar_wait(smem_u32(drained), 0, status, 2);
+  for (int i = 0; i < rows; ++i) column[i * TILE_N] = __uint_as_float(0x7fffffffu);
 }
 
 template <bool kF32>
@@ -251,6 +305,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
     }
     tc::mbar_init(smem_u32(&aux->x_full), 4);
     tc::mbar_init(smem_u32(&aux->ready), 1);  // the owner's arrival + the copied bytes
+    tc::mbar_init(smem_u32(&aux->drained), 3);
+    aux->abort = 0;
     tc::mbar_fence_init();
   }
   tc::fence_before_sync();
@@ -277,6 +333,16 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
   if constexpr (!kFuse) pdl_wait();
   pdl_launch_dependents();
 
+  auto wait = [&](const uint64_t* bar, uint32_t parity) {
+    const uint32_t at = smem_u32(bar);
+    if (tc::mbar_try_wait(at, parity)) return true;
+    if constexpr (kFuse) return wait_loop(at, parity, &aux->abort, a.status, a.wait_limit);
+    else return wait_called(at, parity, &aux->abort, a.status, a.wait_limit);
+  };
+  // The issuers run their loops to the end whatever becomes of a wait: `go`
+  // of the elected lane, which issues, says whether it still does, and a lane
+  // that has given up waits no more.  (A vote and an exit a k-block cost 40
+  // cycles of 630.)
   // a stage's address, barrier and parity advance by counters: a division a
   // k-block showed in the issuers' time
   if (warp == 0) {
@@ -284,7 +350,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
     if (lane == 0) {
       int it = 0, s = 0;
       uint32_t ph = 1;  // parity of the stage's last release
-      for (int item = cid; item < n_items; item += n_cl) {
+      bool go = true;
+      for (int item = cid; go && item < n_items; item += n_cl) {
         const int t = item / a.m_tiles, mt = item - t * a.m_tiles;
         const uint8_t* wt = a.w + (int64_t(t) * a.nkb + kb0) * kWBytes;
         const uint8_t* xt = a.x + (int64_t(mt) * a.nkb + kb0) * x_tile;
@@ -292,7 +359,10 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
           const uint32_t st = sbase + s * a.stage_bytes;
           const uint32_t fb = smem_u32(&aux->full[s]);
           if (it >= npre) {
-            if (it >= NS) tc::mbar_wait(smem_u32(&aux->empty[s]), ph, a.status, 2, a.wait_limit);
+            if (it >= NS && !wait(&aux->empty[s], ph)) {
+              go = false;
+              break;
+            }
             tma::mbar_arrive_expect_tx(fb, stage_tx);
             lin::bulk_load(st, wt, kWBytes, fb);
           }
@@ -303,6 +373,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
           }
         }
       }
+      aux->issued = it;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -312,10 +383,10 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
     const uint32_t sf_step = sf_cols(a.groups), sfb_step = 4 * a.groups;
     int s = 0, li = 0;
     uint32_t ph = 0;
-    if constexpr (kFuse) tc::mbar_wait(smem_u32(&aux->x_full), 0, a.status, 2, a.wait_limit);
+    bool go = !kFuse || wait(&aux->x_full, 0);
     for (int item = cid; item < n_items; item += n_cl, ++li) {
       const int acc = li & 1;
-      if (li >= 2) tc::mbar_wait(smem_u32(&aux->acc_empty[acc]), ((li - 2) >> 1) & 1, a.status, 2, a.wait_limit);
+      if (li >= 2) go = go && wait(&aux->acc_empty[acc], ((li - 2) >> 1) & 1);
       tc::fence_after_sync();
       const uint32_t d = tmem + uint32_t(kMaxBt) * acc;
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -323,10 +394,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
         const uint32_t sfa = tmem + kColSf + sf_step * s, sfb = sfa + 8;
         const uint32_t xt = kFuse ? sbase + a.x_off + (kb - kb0) * x_tile : st + kWBytes;
         const uint32_t a_lo = tc::desc_lo(st, 16), b_lo = tc::desc_lo(xt, 16);
-        tc::mbar_wait(smem_u32(&aux->full[s]), ph, a.status, 2, a.wait_limit);
-        tc::mbar_wait(smem_u32(&aux->sf_full[s]), ph, a.status, 2, a.wait_limit);
+        go = go && wait(&aux->full[s], ph) && wait(&aux->sf_full[s], ph);
         tc::fence_after_sync();
-        if (tc::elect_one()) {
+        if (tc::elect_one() && go) {
 #pragma unroll
           for (int ks = 0; ks < KBW / 64; ++ks)
             tc::mma_mxf4(d, tc::desc_pack(a_lo + ks * 2, hi), tc::desc_pack(b_lo + ks * 2, hi), (ks & 1) ? id2 : id0,
@@ -339,7 +409,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
           ph ^= 1;
         }
       }
-      if (tc::elect_one()) tc::mma_commit(smem_u32(&aux->acc_full[acc]));
+      if (tc::elect_one() && go) tc::mma_commit(smem_u32(&aux->acc_full[acc]));
       __syncwarp();
     }
   } else if (warp == 6) {
@@ -350,16 +420,16 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
     const uint32_t sf_step = sf_cols(a.groups);
     int s = 0;
     uint32_t ph = 0;
-    if constexpr (kFuse) tc::mbar_wait(smem_u32(&aux->x_full), 0, a.status, 2, a.wait_limit);
+    bool go = !kFuse || wait(&aux->x_full, 0);
     for (int item = cid; item < n_items; item += n_cl) {
       for (int kb = kb0; kb < kb1; ++kb) {
         const uint32_t st = sbase + s * a.stage_bytes;
         const uint32_t sfa = tmem + kColSf + sf_step * s;
         const uint32_t xt = kFuse ? sbase + a.x_off + (kb - kb0) * x_tile : st + kWBytes;
         const uint32_t w_lo = tc::desc_lo(st + kCodeBytes, 16), x_lo = tc::desc_lo(xt + x_bytes, 16);
-        tc::mbar_wait(smem_u32(&aux->full[s]), ph, a.status, 2, a.wait_limit);
+        go = go && wait(&aux->full[s], ph);
         tc::fence_after_sync();
-        if (tc::elect_one()) {
+        if (tc::elect_one() && go) {
           tc::cp_scales(sfa, tc::desc_pack(w_lo, hi));
           tc::cp_scales(sfa + 4, tc::desc_pack(w_lo + 32, hi));
           if (a.groups == 1) {
@@ -382,13 +452,15 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
     }
   }
 
-  if (warp >= 2 && warp <= 5) {
+  const bool epilogue = warp >= 2 && warp <= 5;
+  const int quarter = warp & 3;        // TMEM lanes [32 quarter, 32 quarter + 32)
+  const int nr = quarter * 32 + lane;  // this thread's row of the weight tile
+  const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16);
+  uint8_t* stage = smem + a.out_off;
+  const bool lead = tid == 64;
+  bool ok = true;  // given up: through the same barriers, without the stores
+  if (epilogue) {
     // ---------------------------------------------------------------- epilogue (warps 2-5)
-    const int quarter = warp & 3;        // TMEM lanes [32 quarter, 32 quarter + 32)
-    const int nr = quarter * 32 + lane;  // this thread's row of the weight tile
-    const uint32_t trow = tmem + ((uint32_t)(quarter * 32) << 16);
-    uint8_t* stage = smem + a.out_off;
-    const bool lead = tid == 64;
     if (lead && a.tma_store) tma::prefetch_map(&tm_y);
     if constexpr (kFuse) {
       uint8_t* xs = smem + a.x_off;
@@ -413,7 +485,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
           if (lead) lin::bulk_wait_read();
           tc::named_bar_sync(1, 128);
         }
-        tc::mbar_wait(smem_u32(&aux->acc_full[acc]), (li >> 1) & 1, a.status, 2, a.wait_limit);
+        ok = ok && wait(&aux->acc_full[acc], (li >> 1) & 1);
+        __syncwarp();
         tc::fence_after_sync();
         // rows past the tile's tokens are staged too (the store leaves them out)
         const uint32_t tacc = trow + uint32_t(kMaxBt) * acc;
@@ -450,7 +523,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
             if (a.tma_store) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) *stage_at<kF32>(stage, a.half_bytes, c0 + i, nr) = to_out<kF32>(v[i]);
-            } else {
+            } else if (ok) {
               store_rows<kF32, 32>(a, b0 + c0, rows - c0, t * TILE_N + nr, v);
             }
           }
@@ -461,29 +534,38 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
         if (a.tma_store) {
           tc::fence_proxy_async();
           tc::named_bar_sync(1, 128);
-          if (lead) store_tile<kF32>(&tm_y, smem_u32(stage), a.half_bytes, t, int(b0), a.N);
+          if (lead && !*static_cast<volatile int*>(&aux->abort))
+            store_tile<kF32>(&tm_y, smem_u32(stage), a.half_bytes, t, int(b0), a.N);
         }
       }
     } else {
-      tc::mbar_wait(smem_u32(&aux->acc_full[0]), 0, a.status, 2, a.wait_limit);
+      ok = __all_sync(0xffffffffu, wait(&aux->acc_full[0], 0)) != 0;
       tc::fence_after_sync();
     }
+  }
+  if (C > 1) {
+    // one item a cluster; every CTA's products are done once all have arrived
+    lin::cluster_arrive();
+    lin::cluster_wait();
+  }
+  if (epilogue) {
     if (C > 1) {
-      // one item a cluster; every CTA's products are done once all have arrived
-      lin::cluster_arrive();
-      lin::cluster_wait();
       const int t = cid / a.m_tiles, mt = cid - t * a.m_tiles;
       const int64_t b0 = int64_t(mt) * a.Bt;
       const int rows = int(min(int64_t(a.Bt), a.B - b0));
       const int R = a.rows_per, r0 = rank * R, own = max(0, min(rows, r0 + R) - r0);
       float* part = reinterpret_cast<float*>(smem + a.part_off);
       const float* recv = reinterpret_cast<const float*>(smem + a.recv_off);
-      for (int c0 = 0; c0 < rows; c0 += 32) {
-        float v[32];
-        tc::tmem_ld32(trow + c0, v);
-        tc::tmem_wait_ld();
+      if (ok) {
+        for (int c0 = 0; c0 < rows; c0 += 32) {
+          float v[32];
+          tc::tmem_ld32(trow + c0, v);
+          tc::tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) part[(c0 + i) * TILE_N + nr] = v[i];  // (room for whole groups of 32)
+          for (int i = 0; i < 32; ++i) part[(c0 + i) * TILE_N + nr] = v[i];  // (room for whole groups of 32)
+        }
+      } else {
+        poison(part + nr, rows, &aux->drained, a.status);
       }
       tc::fence_proxy_async();  // the copy engine reads the partial
       tc::named_bar_sync(1, 128);
@@ -497,7 +579,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
                             lin::mapa(smem_u32(&aux->ready), q));
         }
       }
-      lin::mbar_wait_cluster(smem_u32(&aux->ready), 0, a.status, a.wait_limit);
+      // every CTA sends, so all copies come: they land before this one leaves
+      if (!lin::mbar_wait_cluster(smem_u32(&aux->ready), 0, a.status, a.wait_limit))
+        ok = lin::mbar_wait_cluster(smem_u32(&aux->ready), 0, a.status, tc::kWaitCycles) && ok;
       for (int l0 = 0; l0 < own; l0 += 8) {
         float v[8];
 #pragma unroll
@@ -509,23 +593,23 @@ __global__ void __launch_bounds__(THREADS, 1) linear_mxfp4_kernel(const Args a,
         if (a.tma_store) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) *stage_at<kF32>(stage, a.half_bytes, l0 + j, nr) = to_out<kF32>(v[j]);
-        } else {
+        } else if (ok) {
           store_rows<kF32, 8>(a, b0 + r0 + l0, own - l0, t * TILE_N + nr, v);
         }
       }
       if (a.tma_store && own > 0) {
         tc::fence_proxy_async();
         tc::named_bar_sync(1, 128);
-        if (lead) store_tile<kF32>(&tm_y, smem_u32(stage), a.half_bytes, t, int(b0) + r0, a.N);
+        if (lead && ok) store_tile<kF32>(&tm_y, smem_u32(stage), a.half_bytes, t, int(b0) + r0, a.N);
       }
     }
     if (lead) lin::bulk_wait_read();  // the tiles have left shared memory
-  } else if (C > 1) {
-    lin::cluster_arrive();
-    lin::cluster_wait();
+  } else if (C > 1 && aux->abort) {
+    drain(aux, NS, a.status);
   }
   tc::fence_before_sync();
   __syncthreads();
+  if (C == 1 && (warp < 2 || warp > 5) && aux->abort) drain(aux, NS, a.status);
   if (C > 1) {  // no CTA leaves while a peer may still touch its shared memory
     lin::cluster_arrive();
     lin::cluster_wait();

@@ -142,7 +142,8 @@ class DeviceLinear:
 
     An MXFP4 weight (mxfp4_parts) stays at 4 bits: the product is
     ``ops.linear_mxfp4``, which quantises x to MXFP4 too and rounds its fp32
-    sums once (``out_dtype=F32``: not at all); ``scale`` must then be 1."""
+    sums once (``out_dtype=F32``: not at all); ``scale`` must then be 1.  Its
+    device status word is ``status`` unless a call brings its own."""
 
     def __init__(self, device, weight, scale: float = 1.0, out_dtype=BF16):
         self.device = _device_of(device)
@@ -165,6 +166,7 @@ class DeviceLinear:
         self.out_dim, self.in_dim = codes.shape[0], 2 * codes.shape[1]
         self.weight = ops.pack_linear_weight_mxfp4(codes.to(self.device).contiguous(),
                                                    scales.to(self.device).contiguous())
+        self.status = torch.zeros(1, dtype=I32, device=self.device)
 
     @classmethod
     def fused(cls, device, weights, names=("kv", "gate")):
@@ -191,6 +193,7 @@ class DeviceLinear:
         lead = x.shape[:-1]
         x2 = x.reshape(-1, self.in_dim).to(BF16).contiguous()
         if isinstance(self.weight, ops.MXFP4Weight):
+            status = self.status if status is None else status
             y = ops.linear_mxfp4(x2, self.weight, out_f32=self.out_dtype != BF16, status=status)
             if rope is not None:
                 cos, sin, pos, head_dim, rope_dim = rope[:5]
