@@ -472,3 +472,25 @@ def test_strides_that_nothing_steps_by(cuda_dev):
     assert torch.equal(ops.kv_quant_read(one, idx), ops.kv_quant_read(want[:1], idx))
     assert torch.equal(ops.sparse_attn_quant(q, one, idx, sink, SCALE),
                        ops.sparse_attn_quant(q, want[:1], idx, sink, SCALE))
+
+
+def test_write_over_every_pair_of_significands(cuda_dev):
+    """Every bf16 significand over the scale of every maximum's, from the
+    maximum down to a code of zero, both signs."""
+    from dsv4attn import ops
+    sig = 1 + torch.arange(128, dtype=torch.float64) / 128
+    x = (sig.view(1, -1) * torch.exp2(-torch.arange(21).double()).view(-1, 1)).flatten()     # 2^0 .. 2^-20 of it
+    x = torch.cat([x, -x, torch.zeros(-2 * x.numel() % 63, dtype=torch.float64)]).view(1, -1, 63)
+    top = (2 * sig).view(-1, 1, 1).expand(-1, x.shape[1], 1)
+    rows = torch.cat([x.expand(128, -1, -1), top], -1).reshape(-1, 64)
+    rows = torch.cat([rows, torch.zeros(-rows.shape[0] % 8, 64, dtype=torch.float64)])
+    for scale in (1.0, 2.0 ** -10, 2.0 ** 90):
+        kv = (rows * scale).to(BF).view(1, -1, 512)
+        assert torch.equal(kv.double().view(-1, 64), rows * scale)
+        n = kv.shape[1]
+        cache = ops.kv_quant_cache(1, n, 512, 0, device=cuda_dev)
+        ops.kv_quant_write(kv.to(cuda_dev), cache, torch.zeros(1, dtype=I32, device=cuda_dev), n, rope_dim=0)
+        codes, s, _ = _want_rows(kv, 0)
+        got, _, gs = ops.kv_quant_views(cache, 512, 0)
+        assert torch.equal(gs.cpu().view(-1), s.view(-1))
+        assert torch.equal(got.cpu().view(U8).view(-1), codes.view(U8).view(-1))

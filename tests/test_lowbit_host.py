@@ -281,3 +281,38 @@ def test_the_module_is_rebuilt_for_another_torch_or_python(monkeypatch, tmp_path
     build.build_torch_ops()
     build.build_torch_ops()
     assert len(ran) == 4
+
+
+def _fl32(v):
+    """The fp32 number nearest to a Fraction, ties to even (no range ends)."""
+    from fractions import Fraction
+    if v == 0:
+        return v
+    a, e = abs(v), 0
+    e = a.numerator.bit_length() - a.denominator.bit_length()
+    if Fraction(2) ** e > a:
+        e -= 1
+    step = Fraction(2) ** (e - 23)
+    n = round(a / step)                                    # (Fraction's round: half to even)
+    return n * step if v > 0 else -n * step
+
+
+def test_the_cache_writes_quotient_is_correctly_rounded():
+    """q = fl(x r), e = fl(q s - x), fl(q - e r) with r = fl(1 / s) is fl(x / s)
+    for every bf16 significand x over every scale s = fl(m fl(1/448)) of a bf16
+    maximum m, and over the smallest scale.  (e is not always exact: q can be
+    more than an ulp off.)"""
+    from fractions import Fraction
+    inv = _fl32(Fraction(1, 448))
+    eps = _fl32(Fraction(1, 10000))
+    scales = [_fl32(Fraction(128 + i, 128) * inv) for i in range(128)] + [_fl32(eps * inv)]
+    inexact = 0
+    for s in scales:
+        r = _fl32(1 / s)
+        for j in range(128):
+            x = Fraction(128 + j, 128)
+            q = _fl32(x * r)
+            e = _fl32(q * s - x)
+            inexact += e != q * s - x
+            assert _fl32(q - e * r) == _fl32(x / s), (x, s)
+    assert inexact == 21                                   # of 129 x 128
