@@ -359,3 +359,63 @@ def test_waits_that_run_out_end_the_call_once(cuda_dev, B, N, K, f32):
         again = ops.linear_mxfp4(x, w, out_f32=f32, status=status)
         torch.cuda.synchronize()
         assert torch.equal(again, want) and int(status) == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("B,N,K", [(1, 1024, 4096), (3, 200, 96), (5, 300, 512), (5, 512, 32768), (48, 130, 256)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_linear_input_types_of_a_few_tokens(cuda_dev, dtype, B, N, K, f32):
+    """The product quantises x itself, of each type, whole and split over K (with
+    owners that have no row)."""
+    from dsv4attn import ops
+    x = torch.randn(B, K, generator=torch.Generator().manual_seed(B + K)).to(dtype)
+    codes, scales = _w(N, K, N)
+    w = ops.pack_linear_weight_mxfp4(codes.to(cuda_dev), scales.to(cuda_dev))
+    _check_linear(ops.linear_mxfp4(x.to(cuda_dev), w, out_f32=f32), x, codes, scales)
+
+
+@pytest.mark.parametrize("B,N,K", [(33, 128, 16384), (40, 130, 16384), (59, 290, 7072), (143, 22, 7424),
+                                   (47, 200, 65536), (100, 130, 29984), (97, 24, 8192)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_linear_split_over_several_token_tiles(cuda_dev, B, N, K, f32):
+    """Splits over K of several token tiles, most of which do not divide the
+    tile: owners with fewer rows or none, no row of the next tile touched."""
+    from dsv4attn import ops
+    x = torch.randn(B, K, generator=torch.Generator().manual_seed(B)).to(BF)
+    codes, scales = _w(N, K, K)
+    w = ops.pack_linear_weight_mxfp4(codes.to(cuda_dev), scales.to(cuda_dev))
+    buf = torch.full((B + 1, N + 8), 7.0, dtype=F32 if f32 else BF, device=cuda_dev)
+    y = ops.linear_mxfp4(x.to(cuda_dev), w, out=buf[:B], out_f32=f32)
+    torch.cuda.synchronize()
+    _check_linear(y[:, :N], x, codes, scales)
+    assert bool((buf[B] == 7.0).all()) and bool((buf[:, N:] == 7.0).all())
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_dev)
+    assert torch.equal(ops.linear_mxfp4(x.to(cuda_dev), w, out_f32=f32, status=status), y[:, :N]) and int(status) == 0
+
+
+def test_quant_of_more_blocks_than_the_grid_holds(cuda_dev):
+    """Every CTA takes a second step (148 SMs x 64 CTAs x 128 blocks)."""
+    from dsv4attn import ops
+    M, K = 10300, 4096
+    x = torch.randn(M, K, generator=torch.Generator(device=cuda_dev).manual_seed(5), device=cuda_dev).to(BF)
+    assert M * K // 32 > 148 * 64 * 128
+    out, scales, codes = ops.mxfp4_quant(x, out=True)
+    pick = [0, 1, M // 2, 9471, 9472, 9473, M - 2, M - 1]  # 148 * 64 * 128 blocks = 9472 rows
+    _check(x[pick].cpu(), (out[pick], scales[pick], codes[pick]))
+    half = M // 2
+    lo, hi = ops.mxfp4_quant(x[:half], out=True), ops.mxfp4_quant(x[half:], out=True)
+    for whole, a, b in zip((out, scales, codes), lo, hi):
+        assert torch.equal(whole[:half], a) and torch.equal(whole[half:], b)
+
+
+@pytest.mark.parametrize("B,N,K", [(40001, 8, 32), (20003, 64, 1056)])
+def test_linear_of_more_tokens_than_the_grid_holds(cuda_dev, B, N, K):
+    """x's quantisation takes a second step a warp (148 SMs x 32 CTAs x 8)."""
+    from dsv4attn import ops
+    assert B * -(-K // 1024) > 148 * 32 * 8
+    x = torch.randn(B, K, generator=torch.Generator().manual_seed(2)).to(BF)
+    codes, scales = _w(N, K, 11)
+    w = ops.pack_linear_weight_mxfp4(codes.to(cuda_dev), scales.to(cuda_dev))
+    y = ops.linear_mxfp4(x.to(cuda_dev), w)
+    pick = torch.cat([torch.arange(40), torch.arange(B // 2, B // 2 + 40), torch.arange(B - 3000, B)])
+    _check_linear(y[pick.to(cuda_dev)], x[pick], codes, scales)
