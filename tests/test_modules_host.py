@@ -113,3 +113,15 @@ def test_device_attention_refuses_mxfp4_weights_of_its_parts(monkeypatch, path):
     if path.startswith("indexer.w"):
         with pytest.raises(ValueError, match="MXFP4"):
             M.DeviceIndexer(torch.device("cpu"), attn.indexer, SimpleNamespace())
+
+
+@pytest.mark.parametrize("scale", [torch.tensor(127, dtype=torch.uint8), torch.full((2,), 127, dtype=torch.uint8),
+                                   torch.full((4, 2, 1), 127, dtype=torch.uint8), torch.full((3, 2), 127, dtype=torch.uint8)])
+def test_an_int8_weight_with_another_kind_of_scale_is_not_mxfp4(scale):
+    """One scale a tensor, or of another shape: an unsupported weight, as before."""
+    from dsv4attn import modules as M
+    w = torch.zeros(4, 32, dtype=torch.int8)
+    w.scale = scale
+    assert M.mxfp4_parts(w) is None
+    w.scale = torch.full((4, 2), 127, dtype=torch.uint8)
+    assert M.mxfp4_parts(w) is not None

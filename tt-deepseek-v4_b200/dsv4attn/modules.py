@@ -92,7 +92,7 @@ def mxfp4_parts(w):
     if scale is None:
         scale = getattr(w, "scale", None)
     if not isinstance(scale, torch.Tensor) or scale.dtype not in (torch.float8_e8m0fnu, torch.uint8) \
-            or 32 * scale.shape[-1] != 2 * t.shape[1]:
+            or scale.dim() != 2 or scale.shape[0] != t.shape[0] or 32 * scale.shape[1] != 2 * t.shape[1]:
         return None
     return t.detach().view(torch.uint8), scale.detach().view(torch.uint8)
 
