@@ -36,8 +36,9 @@
 // MMA time (the product of 4096 x 4096 x 8192: 128 us).  Now a k-block of 192
 // tokens takes ~630, what shared memory moves in that time: 44 KB written by
 // the copies and 40 KB read by the four products at 128 B a cycle.
-// Measured whole: 4096 x 4096 x 8192 79.6 us (3.45 PFLOP/s; x's quantisation
-// ~15 of them), 64 x 32768 x 1024 7.6 us (2.9 TB/s), 1 x 1024 x 4096 4.8 us.
+// Measured whole: 4096 x 4096 x 8192 80.3 us in bursts (3.4 PFLOP/s; x's
+// quantisation ~15 of them; 88-91 back to back, under the power cap), 64 x 32768
+// x 1024 7.7 us (2.9 TB/s), 1 x 1024 x 4096 4.85 us.
 // Tensor memory: 2 x 192 accumulator columns, 128 of scales (8 a stage for W, 8
 // for each 128 tokens of X).
 //
@@ -79,7 +80,7 @@ constexpr int kMaxSplit = 16;
 constexpr int THREADS = 224;
 constexpr int kSmemBytes = 232448;
 constexpr int kAuxBytes = 512;
-constexpr int kFuseUnits = 48;                  // (token, k-block) units of X a CTA quantises itself, at most
+constexpr int kFuseUnits = 32;                  // (token, k-block) units of X a CTA quantises itself, at most
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColSf = 2 * kMaxBt;         // scales of each stage: 8 columns of W, 8 a group of X
 __host__ __device__ constexpr int sf_cols(int groups) { return 8 + 8 * groups; }
@@ -769,8 +770,8 @@ static int lay_out(const Plan& p, int B, int es, bool tma_store, Args* a) {
 // barriers, the exchange of its partial and the sum of C of them.  Half of the
 // time that all bytes would take at 50 a cycle and SM breaks ties towards
 // fewer re-reads.  Measured over 18 shapes x 60 pairs the pick is within 7 % of the
-// best; splitting pays below ~64 tokens (64 x 4096 x 8192: 11.1 us with C = 4,
-// 128 x 4096 x 8192: 15.4 with C = 4, 13.4 unsplit).
+// best; splitting pays below ~64 tokens (64 x 4096 x 8192: 10.6 us with C = 4, 12.7
+// unsplit; 128 x 4096 x 8192: 14.6 with C = 4, 13.7 unsplit).
 static Plan pick_plan(int B, int N, int nkb) {
   static const int kNone[kMaxSplit + 1] = {0, 148};  // no device: unsplit
   const int* clusters = cluster_table();
@@ -808,9 +809,9 @@ static Plan pick_plan(int B, int N, int nkb) {
   }
   // Quantising X in the product saves a launch and X's way through memory and
   // costs each CTA its share of X on four warps.  Measured, fused against two
-  // launches: 1 x 1024 x 4096 (2 units a CTA) 4.8 / 5.7 us, 8 x 1024 x 4096
-  // (16) 5.4 / 6.2, 16 x 1024 x 4096 (32) 6.1 / 6.4, 12 x 32768 x 1024 (48) 6.6 /
-  // 6.8, 24 x 1024 x 4096 (48) 6.8 / 6.5, 16 x 32768 x 1024 (64) 7.2 / 6.8.
+  // launches: 1 x 1024 x 4096 (2 units a CTA) 4.9 / 5.6 us, 8 x 1024 x 4096
+  // (16) 5.45 / 6.1, 16 x 1024 x 4096 (32) 6.3 / 6.3, 12 x 32768 x 1024 (48) 7.0 /
+  // 6.7, 24 x 1024 x 4096 (48) 7.0 / 6.45, 16 x 32768 x 1024 (64) 7.6 / 6.7.
   const int share = (nkb + best.split - 1) / best.split;
   if (best.m_tiles == 1 && int64_t(share) * B <= kFuseUnits) {
     Plan f = best;
