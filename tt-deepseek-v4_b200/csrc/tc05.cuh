@@ -122,8 +122,8 @@ __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.
 // it).  The issuers of tcgen05 instructions run their loops as whole warps and
 // issue under this predicate: their addresses and descriptors are then uniform
 // values of the warp, which inside `if (lane == 0)` they are not.  Measured:
-// attention 35.6 -> 34.8 us (64 x 2176 bf16 rows), MXFP4 projection 12.9 -> 11.0
-// us (333 x 2001 x 4128).
+// attention 36.3 -> 35.5 us (64 x 2176 bf16 rows) and 59-60 -> 53.7 (128 query
+// rows of two sequences), MXFP4 projection 12.9 -> 11.0 us (333 x 2001 x 4128).
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));

@@ -141,8 +141,10 @@ class DeviceLinear:
     DeviceColLinear (inference.py:4954-4966, 5941-5953).
 
     An MXFP4 weight (mxfp4_parts) stays at 4 bits: the product is
-    ``ops.linear_mxfp4``, which quantises x to MXFP4 too and rounds its fp32
-    sums once (``out_dtype=F32``: not at all); ``scale`` must then be 1.  Its
+    ``ops.linear_mxfp4``, which quantises x to MXFP4 too.  The reference expands
+    such a weight and keeps x: against that, y is off by 11-15 % (relative, x of
+    normally distributed elements or of dims of different size); expand the
+    weight to bf16 where that is too much.  The fp32 sums are rounded once (``out_dtype=F32``: not at all); ``scale`` must then be 1.  Its
     device status word is ``status`` unless a call brings its own."""
 
     def __init__(self, device, weight, scale: float = 1.0, out_dtype=BF16):
