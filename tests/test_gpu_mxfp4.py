@@ -419,3 +419,25 @@ def test_linear_of_more_tokens_than_the_grid_holds(cuda_dev, B, N, K):
     y = ops.linear_mxfp4(x.to(cuda_dev), w)
     pick = torch.cat([torch.arange(40), torch.arange(B // 2, B // 2 + 40), torch.arange(B - 3000, B)])
     _check_linear(y[pick.to(cuda_dev)], x[pick], codes, scales)
+
+
+def test_quant_into_columns_beside_its_own(cuda_dev):
+    """x and out as column blocks of one buffer, touching and apart, and as rows
+    one behind the other."""
+    from dsv4attn import ops
+    M, K = 300, 96
+    x = _x(M, K, BF, 9).to(cuda_dev)
+    want = ops.mxfp4_quant(x, out=True)
+    for a, b in ((0, K), (K, 0), (8, 2 * K + 16), (160, 0)):
+        buf = torch.full((2 * M, 400), 7.0, dtype=BF, device=cuda_dev)
+        buf[:M, a:a + K] = x
+        got = ops.mxfp4_quant(buf[:M, a:a + K], out=buf[:M, b:b + K])
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2]) and torch.equal(buf[:M, a:a + K], x)
+        got = ops.mxfp4_quant(buf[:M, a:a + K], out=buf[M:, a:a + K])
+        assert torch.equal(got[0], want[0])
+    with pytest.raises(ValueError, match="overlap"):
+        ops.mxfp4_quant(buf[:M, 0:K], out=buf[1:M + 1, 0:K])
+    one = torch.full((1, 400), 7.0, dtype=BF, device=cuda_dev)
+    one[:, :K] = x[:1]
+    assert torch.equal(ops.mxfp4_quant(one[:, :K], out=one[:, :K])[0], want[0][:1])

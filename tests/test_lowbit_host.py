@@ -316,3 +316,15 @@ def test_the_cache_writes_quotient_is_correctly_rounded():
             inexact += e != q * s - x
             assert _fl32(q - e * r) == _fl32(x / s), (x, s)
     assert inexact == 21                                   # of 129 x 128
+
+
+def test_mxfp4_quant_refuses_an_out_that_partly_covers_x():
+    """out is x itself, a block of columns beside x's, or elsewhere: anything
+    else would overwrite elements that other CTAs have still to read."""
+    from dsv4attn import _lib
+    f = _lib.lib().dsa_mxfp4_quant
+    at, M, K, ld = 1 << 20, 4, 64, 256                     # bf16: rows of 512 B, 128 B of them used
+    for out, ld_out in ((at, ld + 8), (at + 64, ld), (at - 64, ld), (at + 3 * 512 + 112, ld), (at - 3 * 512 - 112, ld),
+                        (at + 512, ld), (at + 400, ld), (at + 128, 64), (at + 1664 - 16, ld)):
+        _refused(f(at, 0, ld, out, ld_out, 16, 16, M, K, None), "overlap")
+    _refused(f(at, 2, 256, at + 256, 256, 16, 16, 2, 128, None), "overlap")   # fp32

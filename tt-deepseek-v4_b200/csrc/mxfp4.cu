@@ -103,6 +103,17 @@ __global__ void __launch_bounds__(kThreads) mxfp4_quant_kernel(const T* x, int64
 
 using namespace dsa;
 
+// out [M rows of `row` bytes, `pitch_o` apart] shares memory with x (`pitch_x`),
+// other than being x, or a block of columns of the same rows beside x's
+static bool partly_covers(const void* x, const void* out, int64_t pitch_x, int64_t pitch_o, int64_t row, int64_t M) {
+  const auto a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(out);
+  if (M == 0 || (a == b && (M == 1 || pitch_x == pitch_o))) return false;
+  if (a + (M - 1) * pitch_x + row <= b || b + (M - 1) * pitch_o + row <= a) return false;
+  if (pitch_x != pitch_o) return true;
+  const int64_t d = int64_t((a > b ? a - b : b - a) % uintptr_t(pitch_x));
+  return d < row || pitch_x - d < row;
+}
+
 extern "C" int dsa_mxfp4_quant(const void* x, int x_type, int64_t ld_x, void* out, int64_t ld_out, uint8_t* codes,
                                uint8_t* scales, int64_t M, int64_t K, dsa_stream_t stream) {
   clear_error();
@@ -115,6 +126,8 @@ extern "C" int dsa_mxfp4_quant(const void* x, int x_type, int64_t ld_x, void* ou
                 "mxfp4_quant: x needs 16-byte alignment and a row stride >= K, a multiple of 16 bytes");
   DSA_CHECK_ARG(!out || (ld_out >= K && ld_out * es % 16 == 0 && aligned(out, 16)),
                 "mxfp4_quant: out needs 16-byte alignment and a row stride >= K, a multiple of 16 bytes");
+  DSA_CHECK_ARG(!out || !partly_covers(x, out, ld_x * es, ld_out * es, K * es, M),
+                "mxfp4_quant: out may be x or lie beside it, not overlap it");
   DSA_CHECK_ARG(aligned(codes, 4), "mxfp4_quant: codes must be 4-byte aligned");
   if (M == 0) return DSA_OK;
   const int64_t blocks = M * (K / mx::kBlock);
